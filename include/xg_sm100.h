@@ -337,6 +337,69 @@ int xg_sdpa_fwd_ws(const void* q, const void* k, const void* v, const void* mask
                    int64_t workspace_bytes, void* stream);
 int64_t xg_sdpa_workspace_bytes(int64_t B, int64_t H, int64_t Sq, int64_t Skv, int64_t D, int dtype);
 
+/* ---- serving from a 4-bit cache ----------------------------------------------------------- */
+
+/*
+ * RMSNorm of every query and key head and the rotary embedding, in one pass:
+ *   y = x * rsqrt(mean(x^2) + eps) * weight over the D channels of a head (a null weight: y = x), then, rotate-half form,
+ *   out_i = y_i cos_i - y_{i+rot/2} sin_i, out_{i+rot/2} = y_{i+rot/2} cos_{i+rot/2} + y_i sin_{i+rot/2} for i < rot/2; channels
+ *   from rot on are y. fp32 arithmetic, rounded once.
+ * q, k: [tokens, heads, D] with element strides per token and head (slices of one packed projection), q_out / k_out contiguous.
+ * cos, sin: contiguous [table_rows, rot]; positions: device, [axes, tokens] with axis_stride elements between axes. With several
+ * axes (time, height, width) the first sections[0] of the rot/2 pairs take their row by axis 0, the next sections[1] by axis 1 and
+ * so on (HOST array, null for one axis). A position outside the table gives zeros. w_dtype, table_dtype: XG_F32 or dtype.
+ * No reference counterpart (its graphs carry the norm and the rotation as separate chains, see xg_rmsnorm and xg_rope).
+ */
+int xg_qk_norm_rope(const void* q, const void* k, const void* q_weight, const void* k_weight, float eps, const void* cos,
+                    const void* sin, int64_t table_rows, int64_t rot, const int64_t* positions, int64_t axes, int64_t axis_stride,
+                    const int64_t* sections, void* q_out, void* k_out, int64_t tokens, int64_t q_heads, int64_t k_heads, int64_t D,
+                    int64_t q_stride_t, int64_t q_stride_h, int64_t k_stride_t, int64_t k_stride_h, int dtype, int w_dtype,
+                    int table_dtype, void* stream);
+
+/*
+ * The 4-bit cache: pages of keys and values. `cache` is device memory, `pages` pages of [heads, page_size / 16] tiles of 18 * D
+ * bytes each, page_stride BYTES apart (a multiple of 16; base 16-byte aligned); page_size is a multiple of 16, D 64, 128 or 256.
+ * A tile holds 16 consecutive tokens of a head: 4-bit codes of keys, of values, then an fp16 (scale, least value) pair per token
+ * and 64 channels of keys, of values; value = code * scale + least. (Places inside a tile: csrc/kv4_tile.cuh.)
+ * A slot is page * page_size + offset.
+ *
+ * xg_kv4_append quantises tokens into slots: least = fp16(min x), scale = fp16((max x - least) / 15), code = rint((x - least) /
+ * scale) in 0..15 per token, head and 64 channels. k, v: [tokens, heads, D] by element strides. Values beyond +-65504 (infinities
+ * too) are held as that, a group with a NaN reads back as NaN. A slot outside the cache (-1, say, for padding rows) is skipped.
+ * Slots are distinct; where two rows share one, that token's contents are unspecified. Nothing else in the cache is touched.
+ * xg_kv4_read writes the slots' values to contiguous [tokens, heads, D]; a slot outside the cache reads as zeros.
+ * xg_copy_pages copies page src[i] to page dst[i], any memory of `pages` pages of page_bytes (a multiple of 16). src, dst: HOST
+ * arrays, checked against `pages`; no page may be a destination twice, or destination and source in one call. 448 pairs a launch.
+ * No reference counterpart.
+ */
+int xg_kv4_append(void* cache, int64_t pages, int64_t heads, int64_t page_size, int64_t page_stride, const void* k, const void* v,
+                  const int64_t* slots, int64_t tokens, int64_t D, int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t,
+                  int64_t v_stride_h, int dtype, void* stream);
+int xg_kv4_read(const void* cache, int64_t pages, int64_t heads, int64_t page_size, int64_t page_stride, const int64_t* slots,
+                int64_t tokens, int64_t D, void* k, void* v, int dtype, void* stream);
+int xg_copy_pages(void* base, int64_t pages, int64_t page_bytes, int64_t page_stride, const int64_t* src, const int64_t* dst,
+                  int64_t count, void* stream);
+
+/*
+ * Attention of the newest tokens of every sequence over its pages: out = softmax(q k^T * scale) v.
+ * q: [tokens, q_heads, D] by element strides per token and head; out: contiguous. Rows q_starts[b] .. q_starts[b+1] (device,
+ * batch + 1 entries; null: row b alone) belong to sequence b, whose kv_lens[b] cached tokens include them: of its n rows, row i
+ * sees the keys up to position kv_lens[b] - n + i. max_q: the most rows that a sequence has; the results do not depend on it, the
+ * choice of the kernel does. Token j of
+ * sequence b lies in page page_table[b * table_stride + j / page_size]; a page number outside the cache hides its keys. q_heads is
+ * a multiple of kv_heads, query head h reads kv head h / (q_heads / kv_heads). Rows that see no key, and rows of no sequence, are
+ * zeros. 16-bit dtypes. All index arrays are int64 device memory. Workspace: xg_kv4_attention_workspace_bytes (max_len =
+ * table_pages * page_size), 16-byte aligned; its contents before and after the call are unspecified.
+ * Reference counterpart: the same aten.scaled_dot_product_attention call site as xg_sdpa_fwd, for a cache it does not have.
+ */
+int64_t xg_kv4_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t D, int64_t max_q,
+                                         int64_t max_len);
+int xg_kv4_attention(const void* q, const void* cache, int64_t pages, int64_t kv_heads, int64_t page_size, int64_t page_stride,
+                     const int64_t* page_table, int64_t table_pages, int64_t table_stride, const int64_t* kv_lens,
+                     const int64_t* q_starts, void* out, int64_t tokens, int64_t batch, int64_t q_heads, int64_t D, int64_t max_q,
+                     int64_t q_stride_t, int64_t q_stride_h, float scale, int dtype, void* workspace, int64_t workspace_bytes,
+                     void* stream);
+
 /* ---- copy fusions (bit-exact) ---------------------------------------------------------- */
 
 /*

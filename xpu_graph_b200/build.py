@@ -35,6 +35,9 @@ SOURCES = [
     "split_bf16x3.cu",
     "pad_rows.cu",
     "sdpa.cu",
+    "qk_norm_rope.cu",
+    "kv4_cache.cu",
+    "kv4_attention.cu",
     "sum3d.cu",
     "rowsum_cat.cu",
 ]

@@ -1,0 +1,266 @@
+// Keys and values in 4 bits: quantising new tokens into cache pages, reading tokens back, copying pages. All three move bytes and
+// are bound by HBM (the layout: kv4_tile.cuh).
+//
+// Quantising, per token, head and group of 64 channels: least = fp16(min x), scale = fp16((max x - least) / 15),
+// code = rint((x - least) / scale) in 0..15, every step in fp32 with IEEE rounding. The fp16 roundings of the pair come first,
+// so the codes are the nearest ones for the pair that is stored.
+#include "kv4_tile.cuh"
+
+namespace xg {
+namespace {
+
+using namespace kv4;
+
+struct TokenParams {
+    Cache cache;
+    const void* k;        // append: values in; read: null
+    const void* v;
+    void* k_out;          // read: values out, [tokens, heads, D]
+    void* v_out;
+    const int64_t* slots;
+    int64_t tokens;
+    int64_t k_st, k_sh, v_st, v_sh;
+};
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+    if (VEC) {
+        constexpr int N = Vec16<T>::N;
+#pragma unroll
+        for (int i = 0; i < 8; i += N) {
+            const Vec16<T> u = ld16_stream(p + i);
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[i + e] = Cvt<T>::to_f(u.v[e]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = Cvt<T>::to_f(p[i]);
+    }
+}
+
+// 8 lanes hold a group's 64 channels: this lane's codes as a word, and the group's pair (scale in the low half).
+__device__ __forceinline__ void quantise(float (&x)[8], uint32_t& word, uint32_t& pair) {
+    float lo = INFINITY, hi = -INFINITY;
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        nan |= x[i] != x[i];
+        x[i] = fminf(fmaxf(x[i], -kLargest), kLargest);
+        lo = fminf(lo, x[i]);
+        hi = fmaxf(hi, x[i]);
+    }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+    // (a shuffle by 1, 2 and 4 stays inside the group's lanes)
+    const uint32_t nans = __ballot_sync(0xffffffffu, nan) >> (threadIdx.x & 24);
+    if (nans & 0xffu) lo = __int_as_float(0x7fffffff);  // a group with a NaN reads back as NaN
+    const __half least = __float2half_rn(lo);
+    const float least_f = __half2float(least);
+    const __half scale = __float2half_rn(__fdiv_rn(hi - least_f, 15.0f));
+    const float scale_f = __half2float(scale);
+    word = 0;
+    if (scale_f > 0.f) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float c = fminf(fmaxf(rintf(__fdiv_rn(x[i] - least_f, scale_f)), 0.f), 15.f);
+            word |= (uint32_t)c << (4 * i);
+        }
+    }
+    pair = (uint32_t)__half_as_ushort(scale) | ((uint32_t)__half_as_ushort(least) << 16);
+}
+
+// A thread takes 8 channels of a token's head, keys and values.
+template <typename T, int D, bool VEC>
+__global__ void __launch_bounds__(256) kv4_append_kernel(const TokenParams p) {
+    pdl_sync();
+    constexpr int J = D / 8;
+    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int j = (int)(at % J);
+    const int64_t th = at / J;
+    const int64_t token = th / p.cache.heads;
+    const int h = (int)(th - token * p.cache.heads);
+    uint8_t* tile = nullptr;
+    int r = 0;
+    float xk[8], xv[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) xk[i] = xv[i] = 0.f;
+    if (token < p.tokens) {  // (a whole group of 8 lanes agrees)
+        const int64_t slot = p.slots[token];
+        load8<T, VEC>(reinterpret_cast<const T*>(p.k) + token * p.k_st + h * p.k_sh + j * 8, xk);
+        load8<T, VEC>(reinterpret_cast<const T*>(p.v) + token * p.v_st + h * p.v_sh + j * 8, xv);
+        tile = const_cast<uint8_t*>(tile_of_slot(p.cache, D, slot, h));
+        r = (int)(slot & 15);
+    }
+    uint32_t wk, pk, wv, pv;
+    quantise(xk, wk, pk);
+    quantise(xv, wv, pv);
+    if (tile == nullptr) return;
+    *reinterpret_cast<uint32_t*>(tile + key_word(D, r, j)) = wk;
+    *reinterpret_cast<uint32_t*>(tile + value_word(D, r, j)) = wv;
+    if ((j & 7) == 0) {
+        *reinterpret_cast<uint32_t*>(tile + pair_at(D, 0, r, j >> 3)) = pk;
+        *reinterpret_cast<uint32_t*>(tile + pair_at(D, 1, r, j >> 3)) = pv;
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_values(T* out, uint32_t word, uint32_t pair) {
+    const float scale = __half2float(__ushort_as_half((unsigned short)(pair & 0xffffu)));
+    const float least = __half2float(__ushort_as_half((unsigned short)(pair >> 16)));
+    constexpr int N = Vec16<T>::N;
+#pragma unroll
+    for (int i = 0; i < 8; i += N) {
+        Vec16<T> u;
+#pragma unroll
+        for (int e = 0; e < N; ++e) u.v[e] = Cvt<T>::from_f(fmaf((float)((word >> (4 * (i + e))) & 15u), scale, least));
+        st16(out + i, u);
+    }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(256) kv4_read_kernel(const TokenParams p) {
+    pdl_sync();
+    constexpr int J = D / 8;
+    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int j = (int)(at % J);
+    const int64_t th = at / J;
+    const int64_t token = th / p.cache.heads;
+    if (token >= p.tokens) return;
+    const int h = (int)(th - token * p.cache.heads);
+    const int64_t slot = p.slots[token];
+    const uint8_t* tile = tile_of_slot(p.cache, D, slot, h);
+    const int r = (int)(slot & 15);
+    uint32_t wk = 0, pk = 0, wv = 0, pv = 0;  // a slot that does not exist reads as zeros
+    if (tile != nullptr) {
+        wk = *reinterpret_cast<const uint32_t*>(tile + key_word(D, r, j));
+        wv = *reinterpret_cast<const uint32_t*>(tile + value_word(D, r, j));
+        pk = *reinterpret_cast<const uint32_t*>(tile + pair_at(D, 0, r, j >> 3));
+        pv = *reinterpret_cast<const uint32_t*>(tile + pair_at(D, 1, r, j >> 3));
+    }
+    store_values(reinterpret_cast<T*>(p.k_out) + th * D + j * 8, wk, pk);
+    store_values(reinterpret_cast<T*>(p.v_out) + th * D + j * 8, wv, pv);
+}
+
+template <typename T, int D>
+int launch_tokens(const TokenParams& p, bool append, cudaStream_t st) {
+    const int64_t threads = p.tokens * p.cache.heads * (D / 8), grid = (threads + 255) / 256;
+    if (grid > 0x7fffffffLL) return fail(XG_ERR_TOO_LARGE, "xg_kv4: too many tokens");
+    if (append) {
+        constexpr int N = Vec16<T>::N;
+        const bool vec = aligned16(p.k) && aligned16(p.v) && p.k_st % N == 0 && p.k_sh % N == 0 && p.v_st % N == 0 && p.v_sh % N == 0;
+        if (vec) launch(kv4_append_kernel<T, D, true>, (unsigned)grid, 256, 0, st, p);
+        else launch(kv4_append_kernel<T, D, false>, (unsigned)grid, 256, 0, st, p);
+        return check_launch("xg_kv4_append");
+    }
+    launch(kv4_read_kernel<T, D>, (unsigned)grid, 256, 0, st, p);
+    return check_launch("xg_kv4_read");
+}
+
+template <typename T>
+int launch_dim(const TokenParams& p, int64_t D, bool append, cudaStream_t st) {
+    switch (D) {
+        case 64: return launch_tokens<T, 64>(p, append, st);
+        case 128: return launch_tokens<T, 128>(p, append, st);
+        default: return launch_tokens<T, 256>(p, append, st);
+    }
+}
+
+int launch_type(const TokenParams& p, int64_t D, int dtype, bool append, cudaStream_t st) {
+    switch (dtype) {
+        case XG_F32: return launch_dim<float>(p, D, append, st);
+        case XG_BF16: return launch_dim<__nv_bfloat16>(p, D, append, st);
+        default: return launch_dim<__half>(p, D, append, st);
+    }
+}
+
+// ---- pages ---------------------------------------------------------------------------------------
+constexpr int kPairs = 448;  // page pairs per launch: with the rest within 4 KiB of kernel parameters
+struct PageParams {
+    uint8_t* base;
+    int64_t page_stride, vectors;  // of 16 bytes in a page
+    int32_t src[kPairs], dst[kPairs];
+};
+static_assert(sizeof(PageParams) <= 4096, "kernel parameters");
+
+constexpr int kCopyVectors = 8;  // in flight per thread
+
+__global__ void __launch_bounds__(256) copy_pages_kernel(const __grid_constant__ PageParams p) {
+    pdl_sync();
+    const uint4* src = reinterpret_cast<const uint4*>(p.base + (int64_t)p.src[blockIdx.y] * p.page_stride);
+    uint4* dst = reinterpret_cast<uint4*>(p.base + (int64_t)p.dst[blockIdx.y] * p.page_stride);
+    const int64_t first = (int64_t)blockIdx.x * (256 * kCopyVectors) + threadIdx.x;
+    uint4 v[kCopyVectors];
+#pragma unroll
+    for (int i = 0; i < kCopyVectors; ++i)
+        if (first + i * 256 < p.vectors) v[i] = src[first + i * 256];
+#pragma unroll
+    for (int i = 0; i < kCopyVectors; ++i)
+        if (first + i * 256 < p.vectors) dst[first + i * 256] = v[i];
+}
+
+}  // namespace
+}  // namespace xg
+
+extern "C" int xg_kv4_append(void* cache, int64_t pages, int64_t heads, int64_t page_size, int64_t page_stride, const void* k, const void* v,
+                             const int64_t* slots, int64_t tokens, int64_t D, int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t,
+                             int64_t v_stride_h, int dtype, void* stream) {
+    using namespace xg;
+    if (const int rc = check_cache("xg_kv4_append", cache, pages, heads, page_size, page_stride, D)) return rc;
+    if (dtype_size(dtype) == 0) return fail(XG_ERR_INVALID_ARG, "xg_kv4_append: bad dtype %d", dtype);
+    if (tokens < 0) return fail(XG_ERR_INVALID_ARG, "xg_kv4_append: bad extents");
+    if (tokens == 0 || pages == 0) return XG_OK;
+    if (!k || !v || !slots) return fail(XG_ERR_INVALID_ARG, "xg_kv4_append: null pointer");
+    TokenParams p = {};
+    p.cache = {static_cast<const uint8_t*>(cache), pages, page_stride, (int)heads, (int)(page_size / 16)};
+    p.k = k; p.v = v; p.slots = slots; p.tokens = tokens;
+    p.k_st = k_stride_t; p.k_sh = k_stride_h; p.v_st = v_stride_t; p.v_sh = v_stride_h;
+    return launch_type(p, D, dtype, true, reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" int xg_kv4_read(const void* cache, int64_t pages, int64_t heads, int64_t page_size, int64_t page_stride, const int64_t* slots,
+                           int64_t tokens, int64_t D, void* k, void* v, int dtype, void* stream) {
+    using namespace xg;
+    if (const int rc = check_cache("xg_kv4_read", cache, pages, heads, page_size, page_stride, D)) return rc;
+    if (dtype_size(dtype) == 0) return fail(XG_ERR_INVALID_ARG, "xg_kv4_read: bad dtype %d", dtype);
+    if (tokens < 0) return fail(XG_ERR_INVALID_ARG, "xg_kv4_read: bad extents");
+    if (tokens == 0) return XG_OK;
+    if (!k || !v || !slots) return fail(XG_ERR_INVALID_ARG, "xg_kv4_read: null pointer");
+    if (!aligned16(k) || !aligned16(v)) return fail(XG_ERR_INVALID_ARG, "xg_kv4_read: results must be 16-byte aligned");
+    TokenParams p = {};
+    p.cache = {static_cast<const uint8_t*>(cache), pages, page_stride, (int)heads, (int)(page_size / 16)};
+    p.k_out = k; p.v_out = v; p.slots = slots; p.tokens = tokens;
+    return launch_type(p, D, dtype, false, reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" int xg_copy_pages(void* base, int64_t pages, int64_t page_bytes, int64_t page_stride, const int64_t* src, const int64_t* dst,
+                             int64_t count, void* stream) {
+    using namespace xg;
+    if (count < 0 || pages < 0 || page_bytes < 0 || (count > 0 && (!src || !dst))) return fail(XG_ERR_INVALID_ARG, "xg_copy_pages: bad arguments");
+    if (pages > 0x7fffffffLL) return fail(XG_ERR_TOO_LARGE, "xg_copy_pages: too many pages");
+    for (int64_t i = 0; i < count; ++i)
+        if (src[i] < 0 || src[i] >= pages || dst[i] < 0 || dst[i] >= pages)
+            return fail(XG_ERR_INVALID_ARG, "xg_copy_pages: page %lld -> %lld outside a cache of %lld pages", (long long)src[i], (long long)dst[i], (long long)pages);
+    if (count == 0 || page_bytes == 0) return XG_OK;
+    if (!base) return fail(XG_ERR_INVALID_ARG, "xg_copy_pages: null pointer");
+    if (!aligned16(base) || page_bytes % 16 != 0 || page_stride % 16 != 0 || (pages > 1 && page_stride < page_bytes))
+        return fail(XG_ERR_UNSUPPORTED, "xg_copy_pages: pages must be multiples of 16 bytes, start on 16-byte boundaries and not overlap");
+    PageParams p;
+    p.base = static_cast<uint8_t*>(base);
+    p.page_stride = page_stride;
+    p.vectors = page_bytes / 16;
+    const int64_t gx = (p.vectors + 256 * kCopyVectors - 1) / (256 * kCopyVectors);
+    if (gx > 0x7fffffffLL) return fail(XG_ERR_TOO_LARGE, "xg_copy_pages: pages too large");
+    for (int64_t at = 0; at < count; at += kPairs) {
+        const int n = (int)(count - at < kPairs ? count - at : kPairs);
+        for (int i = 0; i < n; ++i) {
+            p.src[i] = (int32_t)src[at + i];
+            p.dst[i] = (int32_t)dst[at + i];
+        }
+        launch(copy_pages_kernel, dim3((unsigned)gx, (unsigned)n), 256, 0, reinterpret_cast<cudaStream_t>(stream), p);
+        if (const int rc = check_launch("xg_copy_pages")) return rc;
+    }
+    return XG_OK;
+}

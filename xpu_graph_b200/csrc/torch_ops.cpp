@@ -714,6 +714,161 @@ Tensor sdpa(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const op
     return out;
 }
 
+// ---- serving from a 4-bit cache ------------------------------------------------------------------------------
+// [tokens, heads, D] with contiguous channels; everything else by strides.
+Tensor unit_channels(const Tensor& t) { return t.stride(2) == 1 || t.size(2) == 1 ? t : t.contiguous(); }
+
+void check_index(const char* who, const char* what, const Tensor& t, int64_t dim) {
+    TORCH_CHECK_TYPE(t.scalar_type() == at::kLong, "xg_sm100::", who, ": ", what, " must be int64");
+    TORCH_CHECK_VALUE(t.dim() == dim, "xg_sm100::", who, ": ", what, " must have ", dim, dim == 1 ? " dimension" : " dimensions");
+}
+
+std::vector<Tensor> qk_norm_rope(const Tensor& q_in, const Tensor& k_in, const optional<Tensor>& q_weight, const optional<Tensor>& k_weight, double eps,
+                                 const Tensor& cos_in, const Tensor& sin_in, const Tensor& positions_in, at::IntArrayRef sections) {
+    TORCH_CHECK_VALUE(q_in.dim() == 3 && k_in.dim() == 3 && q_in.size(0) == k_in.size(0) && q_in.size(2) == k_in.size(2),
+                      "xg_sm100::qk_norm_rope expects q and k of [tokens, heads, D] with the same tokens and D");
+    const at::ScalarType dt = q_in.scalar_type();
+    const int64_t T = q_in.size(0), D = q_in.size(2);
+    const int code = code_of(dt);
+    TORCH_CHECK_VALUE(k_in.scalar_type() == dt, "xg_sm100::qk_norm_rope: q and k must share a dtype");
+    TORCH_CHECK_VALUE(D > 0 && (!q_weight || q_weight->numel() == D) && (!k_weight || k_weight->numel() == D),
+                      "xg_sm100::qk_norm_rope: a weight must have one element per channel of a head");
+    TORCH_CHECK_VALUE(cos_in.dim() == 2 && cos_in.sizes() == sin_in.sizes() && cos_in.size(1) % 2 == 0 && cos_in.size(1) <= D,
+                      "xg_sm100::qk_norm_rope: cos and sin must be [positions, rotated channels] with an even number of at most D channels");
+    const int64_t axes = sections.empty() ? 1 : (int64_t)sections.size(), rot = cos_in.size(1);
+    check_index("qk_norm_rope", "positions", positions_in, sections.empty() ? 1 : 2);
+    TORCH_CHECK_VALUE(positions_in.size(-1) == T && (sections.empty() || positions_in.size(0) == axes),
+                      "xg_sm100::qk_norm_rope: positions must be [tokens], or [axes, tokens] with an axis per section");
+    int64_t pairs = 0;
+    for (const int64_t s : sections) {
+        TORCH_CHECK_VALUE(s >= 0 && s <= rot / 2, "xg_sm100::qk_norm_rope: a section is a number of pairs");
+        pairs += s;
+    }
+    TORCH_CHECK_VALUE(axes <= 8, "xg_sm100::qk_norm_rope: at most eight sections");
+    TORCH_CHECK_VALUE(sections.empty() || pairs == rot / 2, "xg_sm100::qk_norm_rope: the sections must add up to half the rotated channels");
+    const On on(q_in);
+    one_device("qk_norm_rope", q_in, k_in, q_weight, k_weight, cos_in, sin_in, positions_in);
+    const Tensor q = unit_channels(q_in), k = unit_channels(k_in);
+    Tensor wq, wk;
+    const auto weight = [&](const optional<Tensor>& w) { return w ? coef(*w, dt) : Tensor(); };
+    wq = weight(q_weight);
+    wk = weight(k_weight);
+    if (wq.defined() && wk.defined() && wq.scalar_type() != wk.scalar_type()) {
+        wq = cast(wq, at::kFloat);
+        wk = cast(wk, at::kFloat);
+    }
+    const int wcode = wq.defined() ? code_of(wq.scalar_type()) : (wk.defined() ? code_of(wk.scalar_type()) : code);
+    Tensor cos = coef(cos_in, dt), sin = coef(sin_in, dt);
+    if (cos.scalar_type() != sin.scalar_type()) {
+        cos = cast(cos, at::kFloat);
+        sin = cast(sin, at::kFloat);
+    }
+    const Tensor positions = unit_rows(positions_in);
+    Tensor yq = new_tensor({T, q.size(1), D}, dt, q), yk = new_tensor({T, k.size(1), D}, dt, q);
+    XG_CALL(xg_qk_norm_rope, ptr(q), ptr(k), ptr(wq), ptr(wk), eps, ptr(cos), ptr(sin), cos.size(0), rot, static_cast<const int64_t*>(ptr(positions)),
+            axes, sections.empty() ? 0 : positions.stride(0), sections.empty() ? nullptr : sections.data(), mut(yq), mut(yk), T, q.size(1), k.size(1),
+            D, q.stride(0), q.stride(1), k.stride(0), k.stride(1), code, wcode, code_of(cos.scalar_type()), on.stream);
+    return {yq, yk};
+}
+
+// uint8 [pages, kv heads, page size / 16, 18 D], a page contiguous
+struct Cache4 {
+    int64_t pages, heads, page_size, stride, D;
+    Cache4(const char* who, const Tensor& t) {
+        TORCH_CHECK_TYPE(t.scalar_type() == at::kByte, "xg_sm100::", who, ": the cache must be uint8");
+        TORCH_CHECK_VALUE(t.dim() == 4 && t.size(1) > 0 && t.size(2) > 0 && t.size(3) % 18 == 0,
+                          "xg_sm100::", who, ": the cache must be [pages, kv heads, page size / 16, 18 * head_dim]");
+        pages = t.size(0);
+        heads = t.size(1);
+        page_size = 16 * t.size(2);
+        D = t.size(3) / 18;
+        const int64_t row = t.size(3), head = t.size(2) * row;
+        TORCH_CHECK_VALUE(t.stride(3) == 1 && (t.size(2) == 1 || t.stride(2) == row) && (heads == 1 || t.stride(1) == head) &&
+                              (pages <= 1 || t.stride(0) >= heads * head),
+                          "xg_sm100::", who, ": a page of the cache must be contiguous");
+        stride = pages > 1 ? t.stride(0) : heads * head;
+    }
+};
+
+void kv4_append(const Tensor& cache, const Tensor& k_in, const Tensor& v_in, const Tensor& slots_in) {
+    const Cache4 c("kv4_append", cache);
+    TORCH_CHECK_VALUE(k_in.dim() == 3 && k_in.sizes() == v_in.sizes() && k_in.size(1) == c.heads && k_in.size(2) == c.D,
+                      "xg_sm100::kv4_append: k and v must be [tokens, ", c.heads, ", ", c.D, "] for this cache");
+    TORCH_CHECK_VALUE(k_in.scalar_type() == v_in.scalar_type(), "xg_sm100::kv4_append: k and v must share a dtype");
+    const int code = code_of(k_in.scalar_type());
+    check_index("kv4_append", "slots", slots_in, 1);
+    TORCH_CHECK_VALUE(slots_in.size(0) == k_in.size(0), "xg_sm100::kv4_append: one slot per token");
+    const On on(cache);
+    one_device("kv4_append", cache, k_in, v_in, slots_in);
+    const Tensor k = unit_channels(k_in), v = unit_channels(v_in), slots = slots_in.contiguous();
+    XG_CALL(xg_kv4_append, mut(cache), c.pages, c.heads, c.page_size, c.stride, ptr(k), ptr(v), static_cast<const int64_t*>(ptr(slots)), k.size(0), c.D,
+            k.stride(0), k.stride(1), v.stride(0), v.stride(1), code, on.stream);
+}
+
+std::vector<Tensor> kv4_read(const Tensor& cache, const Tensor& slots_in, at::ScalarType dtype) {
+    const Cache4 c("kv4_read", cache);
+    const int code = code_of(dtype);
+    check_index("kv4_read", "slots", slots_in, 1);
+    const On on(cache);
+    one_device("kv4_read", cache, slots_in);
+    const Tensor slots = slots_in.contiguous();
+    const int64_t T = slots.size(0);
+    Tensor k = new_tensor({T, c.heads, c.D}, dtype, cache), v = new_tensor({T, c.heads, c.D}, dtype, cache);
+    XG_CALL(xg_kv4_read, ptr(cache), c.pages, c.heads, c.page_size, c.stride, static_cast<const int64_t*>(ptr(slots)), T, c.D, mut(k), mut(v), code, on.stream);
+    return {k, v};
+}
+
+Tensor kv4_attention(const Tensor& q_in, const Tensor& cache, const Tensor& table_in, const Tensor& lens_in, const optional<Tensor>& starts_in,
+                     int64_t max_q, double scale) {
+    const Cache4 c("kv4_attention", cache);
+    TORCH_CHECK_VALUE(q_in.dim() == 3 && q_in.size(2) == c.D && q_in.size(1) > 0 && q_in.size(1) % c.heads == 0,
+                      "xg_sm100::kv4_attention: q must be [tokens, heads, ", c.D, "] with a multiple of ", c.heads, " heads for this cache");
+    const int code = code_of(q_in.scalar_type());
+    check_index("kv4_attention", "page_table", table_in, 2);
+    check_index("kv4_attention", "kv_lens", lens_in, 1);
+    const int64_t T = q_in.size(0), B = lens_in.size(0), H = q_in.size(1);
+    TORCH_CHECK_VALUE(table_in.size(0) == B, "xg_sm100::kv4_attention: one row of the page table per sequence");
+    if (starts_in) {
+        check_index("kv4_attention", "q_starts", *starts_in, 1);
+        TORCH_CHECK_VALUE(starts_in->size(0) == B + 1, "xg_sm100::kv4_attention: q_starts must have an entry per sequence and one more");
+    } else {
+        TORCH_CHECK_VALUE(T == B, "xg_sm100::kv4_attention: without q_starts there is one row of q per sequence");
+    }
+    TORCH_CHECK_VALUE(max_q >= 0, "xg_sm100::kv4_attention: max_q is a number of rows");
+    const On on(q_in);
+    one_device("kv4_attention", q_in, cache, table_in, lens_in, starts_in);
+    const Tensor q = unit_channels(q_in), table = unit_rows(table_in), lens = lens_in.contiguous();
+    const Tensor starts = starts_in ? starts_in->contiguous() : Tensor();
+    const int64_t pages = table.size(1);
+    Tensor out = new_tensor({T, H, c.D}, q.scalar_type(), q);
+    const int64_t ws_bytes = xg_kv4_attention_workspace_bytes(T, B, H, c.heads, c.D, max_q, pages * c.page_size);
+    const Tensor ws = ws_bytes > 0 ? new_tensor({ws_bytes}, at::kByte, q) : Tensor();
+    XG_CALL(xg_kv4_attention, ptr(q), ptr(cache), c.pages, c.heads, c.page_size, c.stride, static_cast<const int64_t*>(ptr(table)), pages,
+            B > 1 ? table.stride(0) : pages, static_cast<const int64_t*>(ptr(lens)), static_cast<const int64_t*>(ptr(starts)), mut(out), T, B, H, c.D, max_q,
+            q.stride(0), q.stride(1), scale, code, mut(ws), ws_bytes, on.stream);
+    return out;
+}
+
+void copy_pages(const Tensor& cache, at::IntArrayRef src, at::IntArrayRef dst) {
+    TORCH_CHECK_VALUE(cache.dim() >= 1 && src.size() == dst.size(), "xg_sm100::copy_pages expects pages and as many destinations as sources");
+    const int64_t pages = cache.size(0);
+    const int64_t bytes = pages > 0 ? cache.numel() / pages * (int64_t)cache.element_size() : 0;
+    TORCH_CHECK_VALUE(pages == 0 || cache.select(0, 0).is_contiguous(), "xg_sm100::copy_pages: a page must be contiguous");
+    const int64_t stride = pages > 1 ? cache.stride(0) * (int64_t)cache.element_size() : bytes;
+    std::vector<char> is_dst(pages, 0);
+    for (const int64_t d : dst) {
+        TORCH_CHECK_VALUE(d >= 0 && d < pages, "xg_sm100::copy_pages: no page ", d, " among ", pages);
+        TORCH_CHECK_VALUE(!is_dst[d], "xg_sm100::copy_pages: page ", d, " is a destination twice");
+        is_dst[d] = 1;
+    }
+    for (const int64_t s : src) {
+        TORCH_CHECK_VALUE(s >= 0 && s < pages, "xg_sm100::copy_pages: no page ", s, " among ", pages);
+        TORCH_CHECK_VALUE(!is_dst[s], "xg_sm100::copy_pages: page ", s, " is source and destination");
+    }
+    const On on(cache);
+    XG_CALL(xg_copy_pages, mut(cache), pages, bytes, stride, src.data(), dst.data(), (int64_t)src.size(), on.stream);
+}
+
 // ---- copy fusions (bit-exact) ------------------------------------------------------------------------------
 struct Segments {
     Buf<const void*> src;
@@ -1246,6 +1401,12 @@ const char* const kSchemas[] = {
     "mlp_small(Tensor x, Tensor[] weights, Tensor?[] biases, str act_names, SymInt weights_kn) -> Tensor",
     "dense_tower(Tensor x, Tensor[] weights, bool[] weight_trans, Tensor?[] biases, str act_names) -> Tensor",
     "sdpa(Tensor q, Tensor k, Tensor v, Tensor? attn_mask, float scale, bool is_causal) -> Tensor",
+    "qk_norm_rope(Tensor q, Tensor k, Tensor? q_weight, Tensor? k_weight, float eps, Tensor cos, Tensor sin, Tensor positions, "
+    "SymInt[] sections) -> Tensor[]",
+    "kv4_append(Tensor(a!) cache, Tensor k, Tensor v, Tensor slots) -> ()",
+    "kv4_read(Tensor cache, Tensor slots, ScalarType dtype) -> Tensor[]",
+    "kv4_attention(Tensor q, Tensor cache, Tensor page_table, Tensor kv_lens, Tensor? q_starts, SymInt max_q, float scale) -> Tensor",
+    "copy_pages(Tensor(a!) cache, SymInt[] src, SymInt[] dst) -> ()",
     "slice_cat(Tensor src, SymInt[] starts, SymInt[] ends, Tensor? row_mask, bool zero_when) -> Tensor",
     "slice_cat_partly_masked(Tensor src, SymInt[] starts, SymInt[] ends, bool[] masked, Tensor row_mask, bool zero_when) -> Tensor",
     "multi_slice(Tensor src, SymInt[] starts, SymInt slice_len) -> Tensor",
@@ -1293,6 +1454,11 @@ TORCH_LIBRARY_IMPL(xg_sm100, CUDA, m) {
     XG_IMPL(mlp_small);
     XG_IMPL(dense_tower);
     XG_IMPL(sdpa);
+    XG_IMPL(qk_norm_rope);
+    XG_IMPL(kv4_append);
+    XG_IMPL(kv4_read);
+    XG_IMPL(kv4_attention);
+    XG_IMPL(copy_pages);
     XG_IMPL(slice_cat);
     XG_IMPL(slice_cat_partly_masked);
     XG_IMPL(multi_slice);

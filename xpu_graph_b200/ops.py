@@ -487,6 +487,61 @@ def _(q, k, v, attn_mask, scale, is_causal):
 
 
 # --------------------------------------------------------------------------------------------
+# serving from a 4-bit cache
+# --------------------------------------------------------------------------------------------
+# RMSNorm of every head of q and k [tokens, heads, D] (a weight of None: no norm) and the rotary embedding, in one pass, rounded
+# once. cos / sin: [positions, R], the first R channels are turned (rotate-half). positions: int64 [tokens], or [axes, tokens]
+# with `sections` = frequency pairs per axis (time, height, width). Returns [q, k], contiguous.
+qk_norm_rope = NativeOp("qk_norm_rope")
+
+
+@qk_norm_rope.register_fake
+def _(q, k, q_weight, k_weight, eps, cos, sin, positions, sections):
+    return [torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)]
+
+
+# The cache of keys and values in 4 bits: uint8 [pages, kv heads, page size / 16, 18 * D], D in {64, 128, 256}; a page may be strided
+# apart from the next. A slot is page * page size + offset.
+# Quantises k, v [tokens, kv heads, D] into `slots` (int64 [tokens], distinct; rows whose slot is not in the cache are skipped).
+kv4_append = NativeOp("kv4_append")
+
+
+@kv4_append.register_fake
+def _(cache, k, v, slots):
+    return None
+
+
+# The values of `slots`, [k, v], each [tokens, kv heads, D].
+kv4_read = NativeOp("kv4_read")
+
+
+@kv4_read.register_fake
+def _(cache, slots, dtype):
+    shape = (slots.shape[0], cache.shape[1], cache.shape[3] // 18)
+    return [torch.empty(shape, dtype=dtype, device=cache.device), torch.empty(shape, dtype=dtype, device=cache.device)]
+
+
+# Attention of the newest tokens over their sequence's pages, causal. q [tokens, heads, D]; rows q_starts[b] .. q_starts[b + 1] are
+# the last of the kv_lens[b] tokens of sequence b (None: one row per sequence), whose page j is page_table[b, j]. max_q: the most
+# rows of a sequence, by which the kernel is chosen. Rows that see no key or belong to no sequence are zeros.
+kv4_attention = NativeOp("kv4_attention")
+
+
+@kv4_attention.register_fake
+def _(q, cache, page_table, kv_lens, q_starts, max_q, scale):
+    return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+
+
+# cache[dst[i]] = cache[src[i]] for pages of any tensor (dimension 0). No page is a destination twice, or source and destination.
+copy_pages = NativeOp("copy_pages")
+
+
+@copy_pages.register_fake
+def _(cache, src, dst):
+    return None
+
+
+# --------------------------------------------------------------------------------------------
 # copy fusions (bit-exact)
 # --------------------------------------------------------------------------------------------
 def _norm_slices(width: int, starts: Sequence[int], ends: Sequence[int]):
