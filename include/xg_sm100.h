@@ -52,8 +52,8 @@ const char* xg_last_error(void);
 /*
  * Status word of the tensor-core kernels on the current device: 0 = healthy; non-zero = a bounded
  * wait inside a kernel expired (bit 0 producer, bit 1 MMA issuer, bit 2 epilogue, bits 4-6 the same
- * roles of the attention kernel, bits 8-10 of the cluster dense kernel, bits 16-18 of the chained-layer kernel, bits 24-25
- * of the fp32 FMA kernel) and that launch's output is invalid. This is the one entry point
+ * roles of the attention kernel, bits 8-10 of the cluster dense kernel, bits 16-18 of the chained-layer kernel, bits 20-23
+ * of the attention over a 4-bit cache, bits 24-25 of the fp32 FMA kernel) and that launch's output is invalid. This is the one entry point
  * that synchronises (it copies the word back); reset != 0 clears it. No reference counterpart.
  */
 int xg_tc_status(unsigned int* status, int reset);

@@ -371,6 +371,8 @@ def test_refusals(cuda_device):
     refused(ValueError, ops.copy_pages, cache, [1], [1])
     refused(ValueError, ops.copy_pages, cache, [4], [0])
     refused(ValueError, ops.copy_pages, cache, [0], [-1])
+    refused(ValueError, ops.copy_pages, cache, slots[:1], slots[1:2])
+    refused(TypeError, ops.copy_pages, cache, torch.zeros(1), torch.ones(1))
     refused(lib.XgLibraryError, ops.copy_pages, torch.zeros(4, 3, dtype=torch.uint8, device=dev), [0], [1])
     assert not cache.any()
 
@@ -455,12 +457,13 @@ def test_operators_compile(cuda_device):
     k, slots = torch.randn(4, 1, 64, device=cuda_device), torch.arange(4, device=cuda_device)
     q, lens = torch.randn(1, 2, 64, device=cuda_device).half(), torch.tensor([4], device=cuda_device)
 
-    def f(cache, k, slots, q, lens):
+    def f(cache, k, slots, q, lens, pages):
         torch.ops.xg_sm100.kv4_append(cache, k, k, slots)
-        torch.ops.xg_sm100.copy_pages(cache, [0], [1])
+        torch.ops.xg_sm100.copy_pages(cache, pages[:1], pages[1:])
         return torch.ops.xg_sm100.kv4_attention(q, cache, slots[1:2, None], lens, None, 1, 0.125) * 2, torch.ops.xg_sm100.kv4_read(cache, slots, torch.float32)[0]
 
+    pages = torch.arange(2)
     other = cache.clone()
-    want = f(cache, k, slots, q, lens)
-    got = torch.compile(f, backend="aot_eager")(other, k, slots, q, lens)
+    want = f(cache, k, slots, q, lens, pages)
+    got = torch.compile(f, backend="aot_eager")(other, k, slots, q, lens, pages)
     assert torch.equal(cache, other) and all(torch.equal(a, b) for a, b in zip(got, want))

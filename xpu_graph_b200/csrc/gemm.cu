@@ -45,6 +45,7 @@ int gemm_f32_group_entry(const void* const* A, const void* const* W, const void*
                          int64_t ldc, int64_t ldr, int trans_b, int act, cudaStream_t st);
 int read_tc_status(unsigned int* host_out, int reset);
 int read_sdpa_status(unsigned int* host_out, int reset);
+int read_kv4_status(unsigned int* host_out, int reset);
 int read_ksplit_status(unsigned int* host_out, int reset);
 int read_mlp_status(unsigned int* host_out, int reset);
 int read_f32_status(unsigned int* host_out, int reset);
@@ -310,6 +311,9 @@ extern "C" int xg_tc_status(unsigned int* status, int reset) {
     unsigned int e = 0;
     rc = xg::read_f32_status(&e, reset);
     if (rc != XG_OK) return rc;
-    *status = a | b | (c << 8) | (d << 16) | (e << 24);
+    unsigned int f = 0;
+    rc = xg::read_kv4_status(&f, reset);
+    if (rc != XG_OK) return rc;
+    *status = a | b | (c << 8) | (d << 16) | (e << 24) | (f << 20);
     return XG_OK;
 }

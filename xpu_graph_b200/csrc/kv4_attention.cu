@@ -4,7 +4,13 @@
 #include "kv4_tile.cuh"
 #include "sm100_ptx.cuh"
 
+#include <type_traits>
+
 namespace xg {
+
+// Status word of the kernels here (device globals are per translation unit without -rdc).
+__device__ unsigned int g_kv4_status[4];
+
 namespace {
 
 using namespace kv4;
@@ -20,6 +26,7 @@ struct AttendParams {
     int64_t q_st, q_sh, table_stride;
     int64_t tokens;
     int batch, heads, group, table_pages;
+    int row0;  // without starts: the row of the first sequence
     float scale;
 };
 
@@ -37,128 +44,683 @@ __device__ __forceinline__ Sequence sequence(const AttendParams& p, int b) {
         s.first = clamp64(p.starts[b], 0, p.tokens);
         end = clamp64(p.starts[b + 1], s.first, p.tokens);
     } else {
-        s.first = b;
-        end = b + 1;
+        s.first = p.row0 + b;
+        end = s.first + 1;
     }
     s.count = (int)(end - s.first);
     s.len = clamp64(p.lens[b], 0, (int64_t)p.table_pages * p.cache.tiles * kTileTokens);
     return s;
 }
 
-// The sequence that row `token` belongs to, -1 if none does.
-__device__ __forceinline__ int sequence_of(const AttendParams& p, int64_t token) {
-    if (!p.starts) return token < p.batch ? (int)token : -1;
-    int lo = 0, hi = p.batch;  // the last b with starts[b] <= token
-    while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (p.starts[mid] <= token) lo = mid + 1;
-        else hi = mid;
-    }
-    if (lo == 0 || p.starts[lo] <= token) return -1;
-    return lo - 1;
+// 8 channels of a finished row; a row that saw no key is zeros.
+template <typename T>
+__device__ __forceinline__ void store_row8(T* out, const float (&o)[8], float sum) {
+    const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
+    Vec16<T> y;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y.v[e] = Cvt<T>::from_f(o[e] * inv);
+    st16(out, y);
 }
 
-// One warp per query token and head: a lane scores a key of 32, then owns D / 32 channels of the output.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) kv4_attend_row_kernel(const AttendParams p) {
+// ---------------------------------------------------------------------------------------
+// Few query rows per sequence: the cache streamed once
+// ---------------------------------------------------------------------------------------
+// A unit is a (sequence, kv head, tile of 8 NT columns); its columns are the (new token, head of the group) pairs that read this kv
+// head. The tiles of 16 keys of all units form one line, cut into equal ranges, one per CTA, so that sequences of any mixture of
+// lengths load the chip evenly; what a unit leaves in several CTAs is added by kv4_combine_kernel in range order. A CTA's warps take
+// its tiles in turn, each warp with a ring of bulk copies of its own.
+//
+// Both products run on mma.m16n8k16 with the codes as bf16: a 4-bit code n masked out of its word is the bf16 subnormal n 2^-133 in
+// bits 0-3 and n 2^-129 in bits 4-7 (8 and up carry over into the exponent as they should), which the tensor core multiplies
+// exactly, so unpacking costs one logic operation per two codes and no arithmetic. q and the probabilities carry 2^64 along.
+//   scores (16 keys x 8 columns, per group of 64 channels):  x = scale_k acc + least_k sum(q), the group's sum of q kept per column
+//   output (16 channels x 8 columns):  acc += code (p scale_v), and the sum of p least_v per column and group beside it
+// p scale_v goes in as two bf16 planes (16 bits of significand), q as one for bf16 and two for fp16 (exact).
+// The maximum is kept per column and may lag behind by 2^8; only a larger step rescales the sums.
+// The codes of keys that do not exist are finite whatever they are; their scales are dropped by a select, not a product.
+constexpr int kWarps = 4, kStages = 3;
+constexpr int kMaxBatch = 1024;  // sequences per launch: their prefix sums live in shared memory
+
+// CTAs per SM, by what the fragments and sums take of the register file
+constexpr int split_ctas(int D, int NT) { return D == 256 ? 2 : (NT == 1 ? 4 : (D == 64 ? 3 : 2)); }
+
+template <int D, int NT>
+struct SplitCfg {
+    static constexpr int COLS = 8 * NT;
+    static constexpr int TILE = tile_bytes(D);
+    static constexpr int RING = kWarps * kStages * TILE;
+    static constexpr int O_STRIDE = D + 4;  // floats
+    static constexpr int O_BYTES = kWarps * COLS * O_STRIDE * 4;
+    static constexpr int ML_BYTES = kWarps * COLS * 2 * 4;
+    static constexpr int BAR_BYTES = kWarps * kStages * 8;
+    static constexpr int FIXED = RING + O_BYTES + ML_BYTES + BAR_BYTES + kWarps * kStages * 4 + 64;
+    static constexpr int part_floats() { return COLS * (D + 2); }
+    static int smem(int batch) { return FIXED + (batch + 1) * 8 + batch * 12; }
+    static constexpr int CTAS = split_ctas(D, NT);
+};
+
+struct SplitParams {
+    AttendParams a;
+    float* parts;  // [2 * gridDim.x][COLS][D] sums, then [2 * gridDim.x][COLS] (maximum, sum) pairs, then a PartDesc per CTA
+    int split;         // 0: a unit stays in one CTA
+    int64_t min_tiles; // of a range
+    int first_rows, last_rows;  // this launch zeroes the rows before the first / behind the last sequence
+};
+
+// What starts in a CTA's range and ends in a later one's.
+struct PartDesc {
+    int parts;  // 0: nothing
+    int first, count, kvh, ct, pad[3];
+};
+
+template <typename T>
+struct Planes {
+    static constexpr int N = std::is_same<T, __nv_bfloat16>::value ? 1 : 2;
+};
+
+template <typename T>
+__device__ __forceinline__ uint4 load_q8(const T* p, bool vec) {  // 8 elements
+    if (vec) return *reinterpret_cast<const uint4*>(p);
+    const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = (uint32_t)h[2 * i] | ((uint32_t)h[2 * i + 1] << 16);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+__device__ __forceinline__ float bf16_lo(uint32_t x) { return __uint_as_float(x << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_split_kernel(const SplitParams sp) {
+    using Cfg = SplitCfg<D, NT>;
+    constexpr int W = D / 32, GR = D / 64, PL = Planes<T>::N;
+    const AttendParams& p = sp.a;
+    extern __shared__ __align__(128) uint8_t smem[];
+    uint8_t* ring = smem;
+    float* o_s = reinterpret_cast<float*>(smem + Cfg::RING);
+    float2* ml_s = reinterpret_cast<float2*>(smem + Cfg::RING + Cfg::O_BYTES);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::RING + Cfg::O_BYTES + Cfg::ML_BYTES);
+    int64_t* prefix = reinterpret_cast<int64_t*>(reinterpret_cast<uint8_t*>(bars) + Cfg::BAR_BYTES);  // [batch + 1]
+    int* first_s = reinterpret_cast<int*>(prefix + p.batch + 1);
+    int* count_s = first_s + p.batch;
+    int* len_s = count_s + p.batch;
+    volatile int* hidden_s = len_s + p.batch;  // [kWarps][kStages]
+    volatile int* abort_flag = hidden_s + kWarps * kStages;
+    int64_t* scan_s = reinterpret_cast<int64_t*>(o_s);  // before the first segment only
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    if (tid == 0) {
+        for (int i = 0; i < kWarps * kStages; ++i) ptx::mbar_init(&bars[i], 1);
+        *abort_flag = 0;
+        ptx::fence_mbar_init();
+        ptx::fence_proxy_async();
+    }
     pdl_sync();
-    __shared__ float q_s[4][D];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t row = (int64_t)blockIdx.x * 4 + warp;
-    const int64_t token = row / p.heads;
-    if (token >= p.tokens) return;
-    const int head = (int)(row - token * p.heads), kvh = head / p.group;
-    T* out = reinterpret_cast<T*>(p.out) + row * D;
-    constexpr int C = D / 32;
-    float o[C];
+
+    // ---- the line of tiles
+    const int kv_heads = p.cache.heads;
+    auto col_tiles = [&](int count) { return (count * p.group + Cfg::COLS - 1) / Cfg::COLS; };
+    auto tiles_of = [&](int b) { return (len_s[b] + kTileTokens - 1) / kTileTokens; };
+    int64_t carry = 0;
+    for (int base = 0; base < p.batch; base += kWarps * 32) {
+        const int b = base + tid;
+        int64_t w = 0;
+        if (b < p.batch) {
+            const Sequence s = sequence(p, b);
+            first_s[b] = (int)s.first;
+            count_s[b] = s.count;
+            len_s[b] = (int)s.len;
+            w = (int64_t)kv_heads * col_tiles(s.count) * ((s.len + kTileTokens - 1) / kTileTokens);
+        }
+        int64_t inc = w;
 #pragma unroll
-    for (int i = 0; i < C; ++i) o[i] = 0.f;
-    float m = -INFINITY, l = 0.f;
-    const int b = sequence_of(p, token);
-    if (b >= 0) {
-        const Sequence s = sequence(p, b);
-        const int64_t visible = s.len - s.count + (token - s.first) + 1;
-        for (int c = lane; c < D; c += 32) q_s[warp][c] = Cvt<T>::to_f(reinterpret_cast<const T*>(p.q)[token * p.q_st + head * p.q_sh + c]);
-        __syncwarp();
-        auto tile_at = [&](int64_t key) -> const uint8_t* {
-            const int64_t t = key >> 4, page = t / p.cache.tiles;
-            const int64_t id = p.table[(int64_t)b * p.table_stride + page];
-            if (id < 0 || id >= p.cache.pages) return nullptr;
-            return p.cache.base + id * p.cache.page_stride + ((int64_t)kvh * p.cache.tiles + (t - page * p.cache.tiles)) * tile_bytes(D);
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += v;
+        }
+        if (lane == 31) scan_s[warp] = inc;
+        __syncthreads();
+        int64_t before = carry, all = carry;
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) {
+            if (i < warp) before += scan_s[i];
+            all += scan_s[i];
+        }
+        if (b < p.batch) prefix[b] = before + inc - w;
+        carry = all;
+        __syncthreads();
+    }
+    if (tid == 0) prefix[p.batch] = carry;
+    __syncthreads();
+    const int64_t total = carry;
+
+    // rows that no key reaches because there is no sequence, or nothing in its cache
+    {
+        const int64_t per_row = (int64_t)p.heads * D;
+        T* out = reinterpret_cast<T*>(p.out);
+        auto zero = [&](int64_t lo, int64_t hi, int first, int step) {
+            for (int64_t r = lo + first; r < hi; r += step)
+                for (int64_t i = tid; i < per_row / 8; i += kWarps * 32) *reinterpret_cast<uint4*>(out + r * per_row + i * 8) = make_uint4(0, 0, 0, 0);
         };
-        auto pair = [&](const uint8_t* tile, int value, int r, int g) {
-            return __half22float2(*reinterpret_cast<const __half2*>(tile + pair_at(D, value, r, g)));
-        };
-        for (int64_t k0 = 0; k0 < visible; k0 += 32) {
-            const int64_t key = k0 + lane;
-            float sc = -INFINITY;
-            if (key < visible) {
-                const uint8_t* tile = tile_at(key);
-                if (tile != nullptr) {
-                    const int r = (int)(key & 15);
-                    sc = 0.f;
-                    for (int g = 0; g < D / 64; ++g) {
-                        const float2 sl = pair(tile, 0, r, g);
-                        for (int j = 8 * g; j < 8 * g + 8; ++j) {
-                            const uint32_t w = *reinterpret_cast<const uint32_t*>(tile + key_word(D, r, j));
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) sc = fmaf(q_s[warp][8 * j + i], fmaf((float)((w >> (4 * i)) & 15u), sl.x, sl.y), sc);
-                        }
-                    }
-                    sc *= p.scale * kLog2e;
-                }
-            }
-            const float m_new = fmaxf(m, warp_max(sc));
-            const float m_use = m_new == -INFINITY ? 0.f : m_new;
-            const float alpha = exp2f(m - m_use), pr = exp2f(sc - m_use);
-            l = l * alpha + warp_sum(pr);
-            m = m_new;
-#pragma unroll
-            for (int i = 0; i < C; ++i) o[i] *= alpha;
-            for (int i = 0; i < 32 && k0 + i < visible; ++i) {
-                const float w = __shfl_sync(0xffffffffu, pr, i);
-                const uint8_t* tile = tile_at(k0 + i);
-                if (tile == nullptr) continue;
-                const int r = (int)((k0 + i) & 15);
-#pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    const int ch = c * 32 + lane;
-                    const uint32_t word = *reinterpret_cast<const uint32_t*>(tile + value_word(D, r, ch >> 3));
-                    const float2 sl = pair(tile, 1, r, ch >> 6);
-                    o[c] = fmaf(w, fmaf((float)((word >> (4 * (ch & 7))) & 15u), sl.x, sl.y), o[c]);
-                }
-            }
+        if (sp.first_rows) zero(0, p.batch > 0 ? first_s[0] : p.tokens, blockIdx.x, gridDim.x);
+        if (sp.last_rows && p.batch > 0) zero((int64_t)first_s[p.batch - 1] + count_s[p.batch - 1], p.tokens, blockIdx.x, gridDim.x);
+        for (int b = blockIdx.x; b < p.batch; b += gridDim.x)
+            if (len_s[b] == 0) zero(first_s[b], (int64_t)first_s[b] + count_s[b], 0, 1);
+    }
+
+    int64_t ranges = (total + sp.min_tiles - 1) / sp.min_tiles;
+    if (ranges > gridDim.x) ranges = gridDim.x;
+    int64_t start = 0, end = 0;
+    auto sequence_at = [&](int64_t x) {  // the b with prefix[b] <= x < prefix[b + 1]
+        int lo = 0, hi = p.batch - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (prefix[mid] <= x) lo = mid;
+            else hi = mid - 1;
+        }
+        return lo;
+    };
+    if ((int64_t)blockIdx.x < ranges) {
+        start = total * blockIdx.x / ranges;
+        end = total * (blockIdx.x + 1) / ranges;
+        if (!sp.split) {
+            auto up = [&](int64_t x) {
+                if (x >= total) return total;
+                const int b = sequence_at(x);
+                const int64_t n = tiles_of(b), off = x - prefix[b];
+                return prefix[b] + (off + n - 1) / n * n;
+            };
+            start = up(start);
+            end = up(end);
         }
     }
-    const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;  // no visible key: zeros
+    PartDesc* desc = reinterpret_cast<PartDesc*>(sp.parts + (int64_t)2 * gridDim.x * Cfg::part_floats()) + blockIdx.x;
+    if (sp.split && tid == 0) desc->parts = 0;
+    if (start >= end) return;
+
+    // ---- this warp's tiles: start + warp + 4 i
+    const int64_t mine = (end - start - warp + kWarps - 1) / kWarps;
+    uint8_t* my_ring = ring + warp * (kStages * Cfg::TILE);
+    uint64_t* my_bars = bars + warp * kStages;
+    volatile int* my_hidden = hidden_s + warp * kStages;
+    int64_t addr = 0;  // this lane's tile of the current batch of 32, 0 where there is none
+    auto issue = [&](int64_t i) {
+        if (i >= mine) return;
+        if ((i & 31) == 0) {
+            const int64_t x = start + warp + (int64_t)kWarps * (i + lane);
+            addr = 0;
+            if (x < end) {
+                const int b = sequence_at(x);
+                const int64_t n = tiles_of(b), off = x - prefix[b];
+                const int64_t unit = off / n;
+                const int tile = (int)(off - unit * n), kvh = (int)(unit / col_tiles(count_s[b]));
+                const int page = tile / p.cache.tiles;
+                const int64_t id = p.table[(int64_t)b * p.table_stride + page];
+                if (id >= 0 && id < p.cache.pages)
+                    addr = reinterpret_cast<int64_t>(p.cache.base + id * p.cache.page_stride + ((int64_t)kvh * p.cache.tiles + (tile - page * p.cache.tiles)) * Cfg::TILE);
+            }
+        }
+        const int64_t from = __shfl_sync(0xffffffffu, addr, (int)(i & 31));
+        const int stage = (int)(i % kStages);
+        if (lane == 0) {
+            my_hidden[stage] = from == 0;
+            if (from != 0) {
+                ptx::mbar_arrive_expect_tx(&my_bars[stage], Cfg::TILE);
+                ptx::bulk_load(my_ring + stage * Cfg::TILE, reinterpret_cast<const void*>(from), Cfg::TILE, &my_bars[stage]);
+            } else {
+                ptx::mbar_arrive(&my_bars[stage]);
+            }
+        }
+    };
+    for (int i = 0; i < kStages; ++i) issue(i);
+
+    const float score_mul = p.scale * kLog2e;
+    const float code_mul = score_mul * 0x1p69f;  // scores: q carries 2^64, codes 2^-133
+    int64_t done = 0;  // tiles of this warp consumed
+    bool ok = true;
+    int b = sequence_at(start);
+    for (int64_t pos = start; pos < end && ok;) {
+        while (prefix[b + 1] <= pos) ++b;
+        const int n_tiles = tiles_of(b), count = count_s[b], len = len_s[b];
+        const int64_t off = pos - prefix[b];
+        const int64_t unit = off / n_tiles;
+        const int t0 = (int)(off - unit * n_tiles);
+        const int cts = col_tiles(count);
+        const int kvh = (int)(unit / cts), ct = (int)(unit - (int64_t)kvh * cts);
+        const int seg = (int)(n_tiles - t0 < end - pos ? n_tiles - t0 : end - pos);
+
+        // ---- q as fragments; column n = 8 nt + g is the pair (new token col / group, head col % group)
+        uint32_t qf[NT][PL][W][4];  // [.][.][w][2 h + i]: fragment register i of k-step 2 w + h
+        float qsum[NT][GR][2];
+        int limit[NT][2];
+        int least_limit = 0x7fffffff;
+        {
+            const T* q = reinterpret_cast<const T*>(p.q);
+            const bool vec = ((reinterpret_cast<uintptr_t>(q) & 15) == 0) && p.q_st % 8 == 0 && p.q_sh % 8 == 0;
 #pragma unroll
-    for (int c = 0; c < C; ++c) out[c * 32 + lane] = Cvt<T>::from_f(o[c] * inv);
+            for (int nt = 0; nt < NT; ++nt) {
+                const int col = ct * Cfg::COLS + nt * 8 + g;
+                const bool on = col < count * p.group;
+                const int token = col / p.group, head = kvh * p.group + (col - token * p.group);
+                const T* row = q + (int64_t)(first_s[b] + token) * p.q_st + (int64_t)head * p.q_sh + 8 * t;
+                uint4 raw[W];
+#pragma unroll
+                for (int w = 0; w < W; ++w) raw[w] = on ? load_q8(row + 32 * w, vec) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                for (int gr = 0; gr < GR; ++gr) {
+                    float sum = 0.f;
+#pragma unroll
+                    for (int w = 2 * gr; w < 2 * gr + 2; ++w) {
+                        float x[8];
+                        const T* e = reinterpret_cast<const T*>(&raw[w]);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            x[i] = Cvt<T>::to_f(e[i]);
+                            sum += x[i];
+                            // odd codes are 16 times as heavy as they should be
+                            x[i] *= (i & 1) ? 0x1p60f : 0x1p64f;
+                        }
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                const float lo = x[2 * h + i], hi = x[2 * h + i + 4];
+                                const uint32_t top = ptx::pack2<__nv_bfloat16>(lo, hi);
+                                qf[nt][0][w][2 * h + i] = top;
+                                if (PL == 2) qf[nt][PL - 1][w][2 * h + i] = ptx::pack2<__nv_bfloat16>(lo - bf16_lo(top), hi - bf16_hi(top));
+                            }
+                    }
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) qsum[nt][gr][c] = score_mul * __shfl_sync(0xffffffffu, sum, (2 * t + c) * 4);
+                }
+                const int lim = on ? len - count + token + 1 : 0x7fffffff;  // keys that the column sees
+                least_limit = min(least_limit, lim);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) limit[nt][c] = __shfl_sync(0xffffffffu, lim, (2 * t + c) * 4);
+            }
+            least_limit = __reduce_min_sync(0xffffffffu, least_limit);
+        }
+        float m[NT][2], l[NT][2], low[NT][GR][2], acc[NT][2 * W][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                m[nt][c] = -INFINITY;
+                l[nt][c] = 0.f;
+#pragma unroll
+                for (int gr = 0; gr < GR; ++gr) low[nt][gr][c] = 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < 2 * W; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[nt][i][e] = 0.f;
+        }
+
+        while (true) {
+            const int64_t x = start + warp + (int64_t)kWarps * done;
+            if (x >= pos + seg) break;
+            const int stage = (int)(done % kStages);
+            if (!__all_sync(0xffffffffu, ptx::mbar_wait_bounded(&my_bars[stage], (uint32_t)((done / kStages) & 1), abort_flag))) { ok = false; break; }
+            const bool hidden = my_hidden[stage] != 0;
+            const int key0 = (t0 + (int)(x - pos)) * kTileTokens;
+            if (!hidden) {
+                const uint8_t* tile = my_ring + stage * Cfg::TILE;
+                // ---- scores
+                uint32_t ka[W], kb[W];
+                const uint8_t* kr = tile + g * (D / 2) + t * (D / 8);
+#pragma unroll
+                for (int w = 0; w < W; w += (W < 4 ? W : 4)) {
+                    if constexpr (W == 2) {
+                        const uint2 a = *reinterpret_cast<const uint2*>(kr), c = *reinterpret_cast<const uint2*>(kr + 4 * D);
+                        ka[0] = a.x; ka[1] = a.y; kb[0] = c.x; kb[1] = c.y;
+                    } else {
+                        const uint4 a = *reinterpret_cast<const uint4*>(kr + 4 * w), c = *reinterpret_cast<const uint4*>(kr + 4 * D + 4 * w);
+                        ka[w] = a.x; ka[w + 1] = a.y; ka[w + 2] = a.z; ka[w + 3] = a.w;
+                        kb[w] = c.x; kb[w + 1] = c.y; kb[w + 2] = c.z; kb[w + 3] = c.w;
+                    }
+                }
+                float sc[NT][4];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sc[nt][e] = 0.f;
+#pragma unroll
+                for (int gr = 0; gr < GR; ++gr) {
+                    float d[NT][4];
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) d[nt][e] = 0.f;
+#pragma unroll
+                    for (int w = 2 * gr; w < 2 * gr + 2; ++w)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t ua = ka[w] >> (8 * h), ub = kb[w] >> (8 * h);
+                            const uint32_t a0 = ua & 0x000f000fu, a1 = ub & 0x000f000fu, a2 = ua & 0x00f000f0u, a3 = ub & 0x00f000f0u;
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int pl = 0; pl < PL; ++pl) ptx::mma_bf16_16816(d[nt], a0, a1, a2, a3, qf[nt][pl][w][2 * h], qf[nt][pl][w][2 * h + 1]);
+                        }
+                    const float2 pa = __half22float2(*reinterpret_cast<const __half2*>(tile + pair_at(D, 0, g, gr)));
+                    const float2 pb = __half22float2(*reinterpret_cast<const __half2*>(tile + pair_at(D, 0, g + 8, gr)));
+                    const float sa = pa.x * code_mul, sb = pb.x * code_mul;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            sc[nt][c] = fmaf(sa, d[nt][c], fmaf(pa.y, qsum[nt][gr][c], sc[nt][c]));
+                            sc[nt][2 + c] = fmaf(sb, d[nt][2 + c], fmaf(pb.y, qsum[nt][gr][c], sc[nt][2 + c]));
+                        }
+                }
+                const bool masked = key0 + kTileTokens > least_limit;  // uniform over the warp
+                if (masked) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (key0 + g + (e & 2) * 4 >= limit[nt][e & 1]) sc[nt][e] = -INFINITY;
+                }
+                // ---- softmax
+                bool grow = false;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) grow = grow || fmaxf(sc[nt][c], sc[nt][2 + c]) > m[nt][c] + 8.f;
+                if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            float mx = fmaxf(sc[nt][c], sc[nt][2 + c]);
+                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                            const float to = fmaxf(m[nt][c], mx);
+                            const float alpha = to == -INFINITY ? 1.f : ptx::ex2_approx(m[nt][c] - to);
+                            m[nt][c] = to;
+                            l[nt][c] *= alpha;
+#pragma unroll
+                            for (int gr = 0; gr < GR; ++gr) low[nt][gr][c] *= alpha;
+#pragma unroll
+                            for (int i = 0; i < 2 * W; ++i) {
+                                acc[nt][i][c] *= alpha;
+                                acc[nt][i][2 + c] *= alpha;
+                            }
+                        }
+                }
+                float pr[NT][4];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float mc = m[nt][e & 1];
+                        pr[nt][e] = ptx::ex2_approx(sc[nt][e] - (mc == -INFINITY ? 0.f : mc));
+                        l[nt][e & 1] += pr[nt][e];
+                    }
+                // ---- output
+                uint32_t v[4][GR];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const uint8_t* vr = tile + 8 * D + (4 * c + t) * (D / 2) + (g ^ (2 * t)) * (D / 16);
+                    if constexpr (GR == 1) {
+                        v[c][0] = *reinterpret_cast<const uint32_t*>(vr);
+                    } else if constexpr (GR == 2) {
+                        const uint2 u = *reinterpret_cast<const uint2*>(vr);
+                        v[c][0] = u.x; v[c][1] = u.y;
+                    } else {
+                        const uint4 u = *reinterpret_cast<const uint4*>(vr);
+                        v[c][0] = u.x; v[c][1] = u.y; v[c][2] = u.z; v[c][3] = u.w;
+                    }
+                }
+#pragma unroll
+                for (int gr = 0; gr < GR; ++gr) {
+                    const float2 pa = __half22float2(*reinterpret_cast<const __half2*>(tile + pair_at(D, 1, g, gr)));
+                    const float2 pb = __half22float2(*reinterpret_cast<const __half2*>(tile + pair_at(D, 1, g + 8, gr)));
+                    const float sa = pa.x * 0x1p64f, sb = pb.x * 0x1p64f;
+                    uint32_t f[NT][2][2];  // [.][plane][keys 0-7, 8-15]
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float w[4], y[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            w[e] = pr[nt][e] * ((e & 2) ? sb : sa);
+                            y[e] = pr[nt][e] * ((e & 2) ? pb.y : pa.y);
+                        }
+                        if (masked) {  // (a hidden key's scale may be anything)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (key0 + g + (e & 2) * 4 >= limit[nt][e & 1]) w[e] = y[e] = 0.f;
+                        }
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) low[nt][gr][c] += y[c] + y[2 + c];
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            const uint32_t top = ptx::pack2<__nv_bfloat16>(w[2 * r], w[2 * r + 1]);
+                            const uint32_t rest = ptx::pack2<__nv_bfloat16>(w[2 * r] - bf16_lo(top), w[2 * r + 1] - bf16_hi(top));
+                            f[nt][0][r] = ptx::transpose_8x8(top);
+                            f[nt][1][r] = ptx::transpose_8x8(rest);
+                        }
+                    }
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const uint32_t u01 = __byte_perm(v[0][gr], v[1][gr], half ? 0x7632 : 0x5410);
+                        const uint32_t u23 = __byte_perm(v[2][gr], v[3][gr], half ? 0x7632 : 0x5410);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t x01 = u01 >> (8 * h), x23 = u23 >> (8 * h);
+                            const uint32_t a0 = x01 & 0x000f000fu, a1 = x01 & 0x00f000f0u, a2 = x23 & 0x000f000fu, a3 = x23 & 0x00f000f0u;
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int pl = 0; pl < 2; ++pl)
+                                    ptx::mma_bf16_16816(acc[nt][4 * gr + 2 * half + h], a0, a1, a2, a3, f[nt][pl][0], f[nt][pl][1]);
+                        }
+                    }
+                }
+            }
+            __syncwarp();  // every lane has read the stage
+            issue(done + kStages);
+            ++done;
+        }
+        if (!ok) break;
+
+        // ---- the warps' sums of this segment together
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) {
+                    l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], o);
+#pragma unroll
+                    for (int gr = 0; gr < GR; ++gr) low[nt][gr][c] += __shfl_xor_sync(0xffffffffu, low[nt][gr][c], o);
+                }
+                if (g == 0) ml_s[warp * Cfg::COLS + nt * 8 + 2 * t + c] = make_float2(m[nt][c], l[nt][c]);
+#pragma unroll
+                for (int i = 0; i < 2 * W; ++i) {  // block i: channels 64 (i / 4) + 8 g + 2 (i % 4) + {0, 1}
+                    const float base = low[nt][i / 4][c];
+                    const float2 y = make_float2(fmaf(acc[nt][i][c], 0x1p69f, base), fmaf(acc[nt][i][2 + c], 0x1p65f, base));
+                    *reinterpret_cast<float2*>(o_s + (warp * Cfg::COLS + nt * 8 + 2 * t + c) * Cfg::O_STRIDE + 64 * (i / 4) + 8 * g + 2 * (i & 3)) = y;
+                }
+            }
+        __syncthreads();
+        if (*abort_flag) { ok = false; break; }
+        const bool whole = seg == n_tiles;
+        const int64_t slot = 2 * (int64_t)blockIdx.x + (t0 == 0 ? 1 : 0);
+        const int cols = min(Cfg::COLS, count * p.group - ct * Cfg::COLS);
+        for (int i = tid; i < cols * (D / 8); i += kWarps * 32) {
+            const int col = i / (D / 8), ch = (i - col * (D / 8)) * 8;
+            float mx = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, ml_s[w * Cfg::COLS + col].x);
+            const float use = mx == -INFINITY ? 0.f : mx;
+            float sum = 0.f, o[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float2 part = ml_s[w * Cfg::COLS + col];
+                const float f = ptx::ex2_approx(part.x - use);
+                sum = fmaf(part.y, f, sum);
+                const float4* src = reinterpret_cast<const float4*>(o_s + (w * Cfg::COLS + col) * Cfg::O_STRIDE + ch);
+                const float4 a = src[0], c = src[1];
+                o[0] = fmaf(a.x, f, o[0]); o[1] = fmaf(a.y, f, o[1]); o[2] = fmaf(a.z, f, o[2]); o[3] = fmaf(a.w, f, o[3]);
+                o[4] = fmaf(c.x, f, o[4]); o[5] = fmaf(c.y, f, o[5]); o[6] = fmaf(c.z, f, o[6]); o[7] = fmaf(c.w, f, o[7]);
+            }
+            if (whole) {
+                const int at = ct * Cfg::COLS + col, token = at / p.group, head = kvh * p.group + (at - token * p.group);
+                store_row8<T>(reinterpret_cast<T*>(p.out) + ((int64_t)(first_s[b] + token) * p.heads + head) * D + ch, o, sum);
+            } else {
+                float4* dst = reinterpret_cast<float4*>(sp.parts + (slot * Cfg::COLS + col) * D + ch);
+                dst[0] = make_float4(o[0], o[1], o[2], o[3]);
+                dst[1] = make_float4(o[4], o[5], o[6], o[7]);
+                if (ch == 0) reinterpret_cast<float2*>(sp.parts + (int64_t)2 * gridDim.x * Cfg::COLS * D)[slot * Cfg::COLS + col] = make_float2(mx, sum);
+            }
+        }
+        if (!whole && t0 == 0 && tid == 0) {  // the unit goes on in the next ranges
+            const int64_t unit_end = pos + n_tiles;
+            int parts = 1;
+            while (total * ((int64_t)blockIdx.x + parts) / ranges < unit_end) ++parts;
+            *desc = {parts, first_s[b], count, kvh, ct, {0, 0, 0}};
+        }
+        __syncthreads();
+        pos += seg;
+    }
+    if (!ok) {  // a copy did not arrive in time: what is in flight gets a bounded time to land before shared memory is given up
+        if (tid == 0) atomicOr(&g_kv4_status[0], 1u);
+        const uint64_t since = ptx::globaltimer_ns();
+        while (ptx::globaltimer_ns() - since < 20000ull) {
+        }
+    }
 }
 
-template <typename T, int D>
-int launch_attend(const AttendParams& p, cudaStream_t st) {
-    const int64_t grid = (p.tokens * p.heads + 3) / 4;
-    if (grid > 0x7fffffffLL) return fail(XG_ERR_TOO_LARGE, "xg_kv4_attention: too many rows");
-    launch(kv4_attend_row_kernel<T, D>, (unsigned)grid, 128, 0, st, p);
+// The parts of the unit that starts in range blockIdx.x and goes on in others: out = sum 2^(m_i - m) O_i / sum 2^(m_i - m) l_i, a CTA
+// per column, its warps take the parts in turn.
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(256) kv4_combine_kernel(const SplitParams sp, int ranges) {
+    using Cfg = SplitCfg<D, NT>;
+    pdl_sync();
+    const PartDesc d = reinterpret_cast<const PartDesc*>(sp.parts + (int64_t)2 * ranges * Cfg::part_floats())[blockIdx.x];
+    const int col = blockIdx.y, at = d.ct * Cfg::COLS + col;
+    if (d.parts == 0 || at >= d.count * sp.a.group) return;
+    __shared__ float o_s[8][D];
+    __shared__ float2 ml_s[8];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const float2* ml = reinterpret_cast<const float2*>(sp.parts + (int64_t)2 * ranges * Cfg::COLS * D);
+    constexpr int C = D / 32;
+    auto slot = [&](int i) { return (i == 0 ? 2 * (int64_t)blockIdx.x + 1 : 2 * ((int64_t)blockIdx.x + i)) * Cfg::COLS + col; };
+    float m = -INFINITY;
+    for (int i = lane; i < d.parts; i += 32) m = fmaxf(m, ml[slot(i)].x);
+    m = warp_max(m);
+    const float use = m == -INFINITY ? 0.f : m;
+    float l = 0.f, o[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) o[c] = 0.f;
+#pragma unroll 4
+    for (int i = warp; i < d.parts; i += 8) {
+        const float2 part = ml[slot(i)];
+        const float f = ptx::ex2_approx(part.x - use);
+        l = fmaf(part.y, f, l);
+        const float* src = sp.parts + slot(i) * D + lane;
+#pragma unroll
+        for (int c = 0; c < C; ++c) o[c] = fmaf(src[c * 32], f, o[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c) o_s[warp][c * 32 + lane] = o[c];
+    if (lane == 0) ml_s[warp].x = l;
+    __syncthreads();
+    const int ch = threadIdx.x * 8;
+    if (ch >= D) return;
+    float sum = 0.f, y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+        sum += ml_s[w].x;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] += o_s[w][ch + e];
+    }
+    const int token = at / sp.a.group, head = d.kvh * sp.a.group + (at - token * sp.a.group);
+    store_row8<T>(reinterpret_cast<T*>(sp.a.out) + ((int64_t)(d.first + token) * sp.a.heads + head) * D + ch, y, sum);
+}
+
+template <typename T, int D, int NT>
+int launch_split(SplitParams sp, cudaStream_t st) {
+    using Cfg = SplitCfg<D, NT>;
+    static std::atomic<uint64_t> reserved;
+    if (!reserve_smem(kv4_split_kernel<T, D, NT>, Cfg::smem(kMaxBatch), reserved)) return fail(XG_ERR_LAUNCH, "xg_kv4_attention: cannot reserve shared memory");
+    const int grid = num_sms() * Cfg::CTAS;
+    launch_with({.early = false}, kv4_split_kernel<T, D, NT>, (unsigned)grid, kWarps * 32, (size_t)Cfg::smem(sp.a.batch), st, sp);
+    if (const int rc = check_launch("xg_kv4_attention")) return rc;
+    if (!sp.split) return XG_OK;
+    launch(kv4_combine_kernel<T, D, NT>, dim3((unsigned)grid, Cfg::COLS), 256, 0, st, sp, grid);
     return check_launch("xg_kv4_attention");
 }
 
+// Columns per unit: what the sequences bring, 16 where they bring more than 8. D = 256 has no registers for 16.
+constexpr int columns(int64_t D, int64_t max_q, int64_t group) { return D == 256 || max_q * group <= 8 ? 8 : 16; }
+
+// Long sequences are cut over CTAs. Short ones are left whole: the second launch and its traffic cost more than uneven ranges.
+constexpr bool cut(int64_t max_len) { return max_len > 1024; }
+
+int64_t split_workspace(int64_t D, int64_t max_q, int64_t group, int64_t max_len) {
+    if (!cut(max_len)) return 0;
+    const int64_t cols = columns(D, max_q, group), ctas = (int64_t)num_sms() * split_ctas((int)D, (int)cols / 8);
+    return 2 * ctas * cols * (D + 2) * 4 + ctas * (int64_t)sizeof(PartDesc);
+}
+
 template <typename T>
-int launch_attend_dim(const AttendParams& p, int64_t D, cudaStream_t st) {
-    switch (D) {
-        case 64: return launch_attend<T, 64>(p, st);
-        case 128: return launch_attend<T, 128>(p, st);
-        default: return launch_attend<T, 256>(p, st);
+int attend_split(const AttendParams& whole, int64_t D, int64_t max_q, void* workspace, cudaStream_t st) {
+    const int64_t max_len = (int64_t)whole.table_pages * whole.cache.tiles * kTileTokens;
+    const int cols = columns(D, max_q, whole.group);
+    for (int at = 0; at == 0 || at < whole.batch; at += kMaxBatch) {
+        SplitParams sp = {};
+        sp.a = whole;
+        sp.a.batch = whole.batch - at < kMaxBatch ? whole.batch - at : kMaxBatch;
+        sp.a.table += (int64_t)at * whole.table_stride;
+        sp.a.lens += at;
+        if (whole.starts) sp.a.starts += at;
+        else sp.a.row0 = at;
+        sp.parts = static_cast<float*>(workspace);
+        sp.split = cut(max_len);
+        sp.min_tiles = 8;
+        sp.first_rows = at == 0;
+        sp.last_rows = at + kMaxBatch >= whole.batch;
+        int rc;
+        if (D == 64) rc = cols == 8 ? launch_split<T, 64, 1>(sp, st) : launch_split<T, 64, 2>(sp, st);
+        else if (D == 128) rc = cols == 8 ? launch_split<T, 128, 1>(sp, st) : launch_split<T, 128, 2>(sp, st);
+        else rc = launch_split<T, 256, 1>(sp, st);
+        if (rc != XG_OK) return rc;
     }
+    return XG_OK;
 }
 
 }  // namespace
+
+int read_kv4_status(unsigned int* host_out, int reset) {
+    unsigned int v[4] = {0, 0, 0, 0};
+    if (cudaMemcpyFromSymbol(v, g_kv4_status, sizeof(v)) != cudaSuccess) {
+        cudaGetLastError();
+        return fail(XG_ERR_DEVICE, "xg_tc_status: cannot read device status");
+    }
+    *host_out = v[0];
+    if (reset && v[0] != 0) {
+        unsigned int z[4] = {0, 0, 0, 0};
+        cudaMemcpyToSymbol(g_kv4_status, z, sizeof(z));
+    }
+    return XG_OK;
+}
 }  // namespace xg
 
 extern "C" int64_t xg_kv4_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t D, int64_t max_q,
                                                     int64_t max_len) {
-    (void)tokens; (void)batch; (void)q_heads; (void)kv_heads; (void)D; (void)max_q; (void)max_len;
-    return 0;
+    using namespace xg;
+    if (tokens <= 0 || batch <= 0 || q_heads <= 0 || kv_heads <= 0 || max_q < 0 || max_len < 0) return 0;
+    return split_workspace(D, max_q, q_heads / kv_heads, max_len);
 }
 
 extern "C" int xg_kv4_attention(const void* q, const void* cache, int64_t pages, int64_t kv_heads, int64_t page_size, int64_t page_stride,
@@ -182,6 +744,9 @@ extern "C" int xg_kv4_attention(const void* q, const void* cache, int64_t pages,
     p.q_st = q_stride_t; p.q_sh = q_stride_h; p.table_stride = table_stride;
     p.tokens = tokens; p.batch = (int)batch; p.heads = (int)q_heads; p.group = (int)(q_heads / kv_heads); p.table_pages = (int)table_pages;
     p.scale = scale;
+    const int64_t need = xg_kv4_attention_workspace_bytes(tokens, batch, q_heads, kv_heads, D, max_q, table_pages * page_size);
+    if (workspace_bytes < need || (need > 0 && (!workspace || !aligned16(workspace))))
+        return fail(XG_ERR_INVALID_ARG, "xg_kv4_attention: needs %lld bytes of 16-byte aligned workspace", (long long)need);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    return dtype == XG_BF16 ? launch_attend_dim<__nv_bfloat16>(p, D, st) : launch_attend_dim<__half>(p, D, st);
+    return dtype == XG_BF16 ? attend_split<__nv_bfloat16>(p, D, max_q, workspace, st) : attend_split<__half>(p, D, max_q, workspace, st);
 }

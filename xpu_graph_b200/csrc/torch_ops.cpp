@@ -849,8 +849,14 @@ Tensor kv4_attention(const Tensor& q_in, const Tensor& cache, const Tensor& tabl
     return out;
 }
 
-void copy_pages(const Tensor& cache, at::IntArrayRef src, at::IntArrayRef dst) {
-    TORCH_CHECK_VALUE(cache.dim() >= 1 && src.size() == dst.size(), "xg_sm100::copy_pages expects pages and as many destinations as sources");
+// The page numbers are host memory: they are checked one by one, and go to the kernel with its launch.
+void copy_pages(const Tensor& cache, const Tensor& src_in, const Tensor& dst_in) {
+    check_index("copy_pages", "src", src_in, 1);
+    check_index("copy_pages", "dst", dst_in, 1);
+    TORCH_CHECK_VALUE(src_in.is_cpu() && dst_in.is_cpu(), "xg_sm100::copy_pages: page numbers must be on the host");
+    TORCH_CHECK_VALUE(cache.dim() >= 1 && src_in.numel() == dst_in.numel(), "xg_sm100::copy_pages expects pages and as many destinations as sources");
+    const Tensor src_t = src_in.contiguous(), dst_t = dst_in.contiguous();
+    const at::IntArrayRef src(src_t.const_data_ptr<int64_t>(), src_t.numel()), dst(dst_t.const_data_ptr<int64_t>(), dst_t.numel());
     const int64_t pages = cache.size(0);
     const int64_t bytes = pages > 0 ? cache.numel() / pages * (int64_t)cache.element_size() : 0;
     TORCH_CHECK_VALUE(pages == 0 || cache.select(0, 0).is_contiguous(), "xg_sm100::copy_pages: a page must be contiguous");
@@ -1406,7 +1412,7 @@ const char* const kSchemas[] = {
     "kv4_append(Tensor(a!) cache, Tensor k, Tensor v, Tensor slots) -> ()",
     "kv4_read(Tensor cache, Tensor slots, ScalarType dtype) -> Tensor[]",
     "kv4_attention(Tensor q, Tensor cache, Tensor page_table, Tensor kv_lens, Tensor? q_starts, SymInt max_q, float scale) -> Tensor",
-    "copy_pages(Tensor(a!) cache, SymInt[] src, SymInt[] dst) -> ()",
+    "copy_pages(Tensor(a!) cache, Tensor src, Tensor dst) -> ()",
     "slice_cat(Tensor src, SymInt[] starts, SymInt[] ends, Tensor? row_mask, bool zero_when) -> Tensor",
     "slice_cat_partly_masked(Tensor src, SymInt[] starts, SymInt[] ends, bool[] masked, Tensor row_mask, bool zero_when) -> Tensor",
     "multi_slice(Tensor src, SymInt[] starts, SymInt slice_len) -> Tensor",

@@ -11,6 +11,7 @@ Registration pattern follows passes/patterns/targets/mlu/triton_kernel/fused_sli
 """
 from __future__ import annotations
 
+import array
 import sys
 import types
 from typing import List, Optional, Sequence
@@ -532,8 +533,22 @@ def _(q, cache, page_table, kv_lens, q_starts, max_q, scale):
     return torch.empty(q.shape, dtype=q.dtype, device=q.device)
 
 
+class _CopyPages(NativeOp):
+    """Page numbers as int64 tensors on the host, or as sequences of ints (an operator's list argument would cost 0.1 us a number)."""
+
+    def __call__(self, cache, src, dst):
+        return self._overload(cache, _host_ints(src), _host_ints(dst))
+
+
+def _host_ints(v) -> torch.Tensor:
+    if isinstance(v, torch.Tensor):
+        return v
+    a = array.array("q", v)
+    return torch.frombuffer(a, dtype=torch.int64) if a else torch.empty(0, dtype=torch.int64)
+
+
 # cache[dst[i]] = cache[src[i]] for pages of any tensor (dimension 0). No page is a destination twice, or source and destination.
-copy_pages = NativeOp("copy_pages")
+copy_pages = _CopyPages("copy_pages")
 
 
 @copy_pages.register_fake
