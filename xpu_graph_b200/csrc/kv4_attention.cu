@@ -79,21 +79,25 @@ __device__ __forceinline__ void store_row8(T* out, const float (&o)[8], float su
 // The maximum is kept per column and may lag behind by 2^8; only a larger step rescales the sums.
 // The codes of keys that do not exist are finite whatever they are; their scales are dropped by a select, not a product.
 constexpr int kWarps = 4, kStages = 3;
+constexpr int kBlockTiles = 2, kBlockKeys = kBlockTiles * kTileTokens;  // what a stage holds
 constexpr int kMaxBatch = 1024;  // sequences per launch: their prefix sums live in shared memory
 
 // CTAs per SM, by what the fragments and sums take of the register file
-constexpr int split_ctas(int D, int NT) { return D == 256 ? 2 : (NT == 1 ? 4 : (D == 64 ? 3 : 2)); }
+constexpr int split_ctas(int D, int NT) { return D == 256 ? 2 : (NT == 1 ? (D == 64 ? 4 : 3) : (D == 64 ? 3 : 2)); }
 
 template <int D, int NT>
 struct SplitCfg {
     static constexpr int COLS = 8 * NT;
     static constexpr int TILE = tile_bytes(D);
-    static constexpr int RING = kWarps * kStages * TILE;
+    static constexpr int STAGE = kBlockTiles * TILE;
+    static constexpr int STAGES = D == 256 ? 2 : kStages;
+    static constexpr int KT = NT == 1 && D <= 128 ? 2 : 1;  // tiles in work at once: more independent products per warp, more registers
+    static constexpr int RING = kWarps * STAGES * STAGE;
     static constexpr int O_STRIDE = D + 4;  // floats
     static constexpr int O_BYTES = kWarps * COLS * O_STRIDE * 4;
     static constexpr int ML_BYTES = kWarps * COLS * 2 * 4;
-    static constexpr int BAR_BYTES = kWarps * kStages * 8;
-    static constexpr int FIXED = RING + O_BYTES + ML_BYTES + BAR_BYTES + kWarps * kStages * 4 + 64;
+    static constexpr int BAR_BYTES = kWarps * STAGES * 8;
+    static constexpr int FIXED = RING + O_BYTES + ML_BYTES + BAR_BYTES + kWarps * STAGES * 4 + 64;
     static constexpr int part_floats() { return COLS * (D + 2); }
     static int smem(int batch) { return FIXED + (batch + 1) * 8 + batch * 12; }
     static constexpr int CTAS = split_ctas(D, NT);
@@ -103,7 +107,7 @@ struct SplitParams {
     AttendParams a;
     float* parts;  // [2 * gridDim.x][COLS][D] sums, then [2 * gridDim.x][COLS] (maximum, sum) pairs, then a PartDesc per CTA
     int split;         // 0: a unit stays in one CTA
-    int64_t min_tiles; // of a range
+    int64_t min_blocks; // of a range
     int first_rows, last_rows;  // this launch zeroes the rows before the first / behind the last sequence
 };
 
@@ -131,6 +135,37 @@ __device__ __forceinline__ uint4 load_q8(const T* p, bool vec) {  // 8 elements
 __device__ __forceinline__ float bf16_lo(uint32_t x) { return __uint_as_float(x << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
 
+// N 32-bit words at once
+template <int N>
+__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&out)[N]) {
+    if constexpr (N == 1) {
+        out[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else if constexpr (N == 2) {
+        const uint2 u = *reinterpret_cast<const uint2*>(p);
+        out[0] = u.x; out[1] = u.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const uint4 u = *reinterpret_cast<const uint4*>(p + 4 * i);
+            out[i] = u.x; out[i + 1] = u.y; out[i + 2] = u.z; out[i + 3] = u.w;
+        }
+    }
+}
+// N (scale, least) pairs at once
+template <int N>
+__device__ __forceinline__ void load_pairs(const uint8_t* p, __half2 (&out)[N]) {
+    uint32_t u[N];
+    load_words<N>(p, u);
+#pragma unroll
+    for (int i = 0; i < N; ++i) out[i] = *reinterpret_cast<const __half2*>(&u[i]);
+}
+
+// The usual case is one question; what waits longer does so outside the loop's code.
+__device__ __noinline__ bool wait_longer(uint64_t* bar, uint32_t phase, volatile int* abort_flag) { return ptx::mbar_wait_bounded(bar, phase, abort_flag); }
+__device__ __forceinline__ bool wait_stage(uint64_t* bar, uint32_t phase, volatile int* abort_flag) {
+    return ptx::mbar_try_wait(bar, phase) || wait_longer(bar, phase, abort_flag);
+}
+
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_split_kernel(const SplitParams sp) {
     using Cfg = SplitCfg<D, NT>;
@@ -145,13 +180,13 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
     int* first_s = reinterpret_cast<int*>(prefix + p.batch + 1);
     int* count_s = first_s + p.batch;
     int* len_s = count_s + p.batch;
-    volatile int* hidden_s = len_s + p.batch;  // [kWarps][kStages]
-    volatile int* abort_flag = hidden_s + kWarps * kStages;
+    volatile int* hidden_s = len_s + p.batch;  // [kWarps][STAGES], a bit per tile
+    volatile int* abort_flag = hidden_s + kWarps * Cfg::STAGES;
     int64_t* scan_s = reinterpret_cast<int64_t*>(o_s);  // before the first segment only
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     if (tid == 0) {
-        for (int i = 0; i < kWarps * kStages; ++i) ptx::mbar_init(&bars[i], 1);
+        for (int i = 0; i < kWarps * Cfg::STAGES; ++i) ptx::mbar_init(&bars[i], 1);
         *abort_flag = 0;
         ptx::fence_mbar_init();
         ptx::fence_proxy_async();
@@ -161,7 +196,7 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
     // ---- the line of tiles
     const int kv_heads = p.cache.heads;
     auto col_tiles = [&](int count) { return (count * p.group + Cfg::COLS - 1) / Cfg::COLS; };
-    auto tiles_of = [&](int b) { return (len_s[b] + kTileTokens - 1) / kTileTokens; };
+    auto blocks_of = [&](int b) { return (len_s[b] + kBlockKeys - 1) / kBlockKeys; };
     int64_t carry = 0;
     for (int base = 0; base < p.batch; base += kWarps * 32) {
         const int b = base + tid;
@@ -171,7 +206,7 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
             first_s[b] = (int)s.first;
             count_s[b] = s.count;
             len_s[b] = (int)s.len;
-            w = (int64_t)kv_heads * col_tiles(s.count) * ((s.len + kTileTokens - 1) / kTileTokens);
+            w = (int64_t)kv_heads * col_tiles(s.count) * ((s.len + kBlockKeys - 1) / kBlockKeys);
         }
         int64_t inc = w;
 #pragma unroll
@@ -209,7 +244,7 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
             if (len_s[b] == 0) zero(first_s[b], (int64_t)first_s[b] + count_s[b], 0, 1);
     }
 
-    int64_t ranges = (total + sp.min_tiles - 1) / sp.min_tiles;
+    int64_t ranges = (total + sp.min_blocks - 1) / sp.min_blocks;
     if (ranges > gridDim.x) ranges = gridDim.x;
     int64_t start = 0, end = 0;
     auto sequence_at = [&](int64_t x) {  // the b with prefix[b] <= x < prefix[b + 1]
@@ -228,7 +263,7 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
             auto up = [&](int64_t x) {
                 if (x >= total) return total;
                 const int b = sequence_at(x);
-                const int64_t n = tiles_of(b), off = x - prefix[b];
+                const int64_t n = blocks_of(b), off = x - prefix[b];
                 return prefix[b] + (off + n - 1) / n * n;
             };
             start = up(start);
@@ -240,55 +275,74 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
     if (start >= end) return;
 
     // ---- this warp's tiles: start + warp + 4 i
-    const int64_t mine = (end - start - warp + kWarps - 1) / kWarps;
-    uint8_t* my_ring = ring + warp * (kStages * Cfg::TILE);
-    uint64_t* my_bars = bars + warp * kStages;
-    volatile int* my_hidden = hidden_s + warp * kStages;
-    int64_t addr = 0;  // this lane's tile of the current batch of 32, 0 where there is none
-    auto issue = [&](int64_t i) {
-        if (i >= mine) return;
-        if ((i & 31) == 0) {
-            const int64_t x = start + warp + (int64_t)kWarps * (i + lane);
-            addr = 0;
-            if (x < end) {
-                const int b = sequence_at(x);
-                const int64_t n = tiles_of(b), off = x - prefix[b];
-                const int64_t unit = off / n;
-                const int tile = (int)(off - unit * n), kvh = (int)(unit / col_tiles(count_s[b]));
-                const int page = tile / p.cache.tiles;
-                const int64_t id = p.table[(int64_t)b * p.table_stride + page];
-                if (id >= 0 && id < p.cache.pages)
-                    addr = reinterpret_cast<int64_t>(p.cache.base + id * p.cache.page_stride + ((int64_t)kvh * p.cache.tiles + (tile - page * p.cache.tiles)) * Cfg::TILE);
-            }
+    const int mine = (int)((end - start - warp + kWarps - 1) / kWarps);
+    uint8_t* my_ring = ring + warp * (Cfg::STAGES * Cfg::STAGE);
+    uint64_t* my_bars = bars + warp * Cfg::STAGES;
+    volatile int* my_hidden = hidden_s + warp * Cfg::STAGES;
+    // where this lane's block of the current batch of 32 lies, tile by tile; 0 where there is nothing to read
+    int64_t addr[kBlockTiles] = {};
+    auto look_up = [&](int i) {
+        const int64_t x = start + warp + (int64_t)kWarps * (i + lane);
+#pragma unroll
+        for (int k = 0; k < kBlockTiles; ++k) addr[k] = 0;
+        if (x >= end) return;
+        const int b = sequence_at(x);
+        const int64_t n = blocks_of(b), off = x - prefix[b];
+        const int64_t unit = off / n;
+        const int kvh = (int)(unit / col_tiles(count_s[b]));
+#pragma unroll
+        for (int k = 0; k < kBlockTiles; ++k) {
+            const int tile = (int)(off - unit * n) * kBlockTiles + k;
+            if (tile * kTileTokens >= len_s[b]) break;
+            const int page = tile / p.cache.tiles;
+            const int64_t id = p.table[(int64_t)b * p.table_stride + page];
+            if (id >= 0 && id < p.cache.pages)
+                addr[k] = reinterpret_cast<int64_t>(p.cache.base + id * p.cache.page_stride + ((int64_t)kvh * p.cache.tiles + (tile - page * p.cache.tiles)) * Cfg::TILE);
         }
-        const int64_t from = __shfl_sync(0xffffffffu, addr, (int)(i & 31));
-        const int stage = (int)(i % kStages);
+    };
+    auto issue = [&](int i, int stage) {
+        if (i >= mine) return;
+        if ((i & 31) == 0) look_up(i);
+        int64_t from[kBlockTiles];
+#pragma unroll
+        for (int k = 0; k < kBlockTiles; ++k) from[k] = __shfl_sync(0xffffffffu, addr[k], i & 31);
         if (lane == 0) {
-            my_hidden[stage] = from == 0;
-            if (from != 0) {
-                ptx::mbar_arrive_expect_tx(&my_bars[stage], Cfg::TILE);
-                ptx::bulk_load(my_ring + stage * Cfg::TILE, reinterpret_cast<const void*>(from), Cfg::TILE, &my_bars[stage]);
+            int hidden = 0, bytes = 0;
+#pragma unroll
+            for (int k = 0; k < kBlockTiles; ++k) {
+                if (from[k] == 0) hidden |= 1 << k;
+                else bytes += Cfg::TILE;
+            }
+            my_hidden[stage] = hidden;
+            ptx::mbar_arrive_expect_tx(&my_bars[stage], bytes);
+            if (from[1] == from[0] + Cfg::TILE) {
+                ptx::bulk_load(my_ring + stage * Cfg::STAGE, reinterpret_cast<const void*>(from[0]), 2 * Cfg::TILE, &my_bars[stage]);
             } else {
-                ptx::mbar_arrive(&my_bars[stage]);
+#pragma unroll
+                for (int k = 0; k < kBlockTiles; ++k)
+                    if (from[k] != 0) ptx::bulk_load(my_ring + stage * Cfg::STAGE + k * Cfg::TILE, reinterpret_cast<const void*>(from[k]), Cfg::TILE, &my_bars[stage]);
             }
         }
     };
-    for (int i = 0; i < kStages; ++i) issue(i);
+    for (int i = 0; i < Cfg::STAGES; ++i) issue(i, i);
 
-    const float score_mul = p.scale * kLog2e;
-    const float code_mul = score_mul * 0x1p69f;  // scores: q carries 2^64, codes 2^-133
-    int64_t done = 0;  // tiles of this warp consumed
+    // Scores stay in the units of the products (2^-69 / scale) up to the exponent; a negative scale goes into q, a zero one makes q zero.
+    const float q_mul = p.scale > 0.f ? 1.f : (p.scale < 0.f ? -1.f : (p.scale == 0.f ? 0.f : p.scale));
+    const float to_log2 = (p.scale != 0.f ? fabsf(p.scale) : 1.f) * kLog2e * 0x1p69f;
+    const float step = 8.f / to_log2;
+    int done = 0, stage = 0;  // tiles of this warp consumed, and the stage of the next one
+    uint32_t phase = 0;
     bool ok = true;
     int b = sequence_at(start);
     for (int64_t pos = start; pos < end && ok;) {
         while (prefix[b + 1] <= pos) ++b;
-        const int n_tiles = tiles_of(b), count = count_s[b], len = len_s[b];
+        const int n_blocks = blocks_of(b), count = count_s[b], len = len_s[b];
         const int64_t off = pos - prefix[b];
-        const int64_t unit = off / n_tiles;
-        const int t0 = (int)(off - unit * n_tiles);
+        const int64_t unit = off / n_blocks;
+        const int t0 = (int)(off - unit * n_blocks);  // blocks, as n_blocks and seg
         const int cts = col_tiles(count);
         const int kvh = (int)(unit / cts), ct = (int)(unit - (int64_t)kvh * cts);
-        const int seg = (int)(n_tiles - t0 < end - pos ? n_tiles - t0 : end - pos);
+        const int seg = (int)(n_blocks - t0 < end - pos ? n_blocks - t0 : end - pos);
 
         // ---- q as fragments; column n = 8 nt + g is the pair (new token col / group, head col % group)
         uint32_t qf[NT][PL][W][4];  // [.][.][w][2 h + i]: fragment register i of k-step 2 w + h
@@ -316,7 +370,7 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
                         const T* e = reinterpret_cast<const T*>(&raw[w]);
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
-                            x[i] = Cvt<T>::to_f(e[i]);
+                            x[i] = Cvt<T>::to_f(e[i]) * q_mul;
                             sum += x[i];
                             // odd codes are 16 times as heavy as they should be
                             x[i] *= (i & 1) ? 0x1p60f : 0x1p64f;
@@ -334,7 +388,7 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
                     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) qsum[nt][gr][c] = score_mul * __shfl_sync(0xffffffffu, sum, (2 * t + c) * 4);
+                    for (int c = 0; c < 2; ++c) qsum[nt][gr][c] = 0x1p-69f * __shfl_sync(0xffffffffu, sum, (2 * t + c) * 4);
                 }
                 const int lim = on ? len - count + token + 1 : 0x7fffffff;  // keys that the column sees
                 least_limit = min(least_limit, lim);
@@ -343,12 +397,14 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
             }
             least_limit = __reduce_min_sync(0xffffffffu, least_limit);
         }
-        float m[NT][2], l[NT][2], low[NT][GR][2], acc[NT][2 * W][4];
+        // m: largest score; bar: what a score has to exceed for m to follow; use: the exponent's offset. Probabilities carry 2^64.
+        float m[NT][2], bar[NT][2], use[NT][2], l[NT][2], low[NT][GR][2], acc[NT][2 * W][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                m[nt][c] = -INFINITY;
+                m[nt][c] = bar[nt][c] = -INFINITY;
+                use[nt][c] = 64.f;
                 l[nt][c] = 0.f;
 #pragma unroll
                 for (int gr = 0; gr < GR; ++gr) low[nt][gr][c] = 0.f;
@@ -359,144 +415,154 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
                 for (int e = 0; e < 4; ++e) acc[nt][i][e] = 0.f;
         }
 
-        while (true) {
-            const int64_t x = start + warp + (int64_t)kWarps * done;
-            if (x >= pos + seg) break;
-            const int stage = (int)(done % kStages);
-            if (!__all_sync(0xffffffffu, ptx::mbar_wait_bounded(&my_bars[stage], (uint32_t)((done / kStages) & 1), abort_flag))) { ok = false; break; }
-            const bool hidden = my_hidden[stage] != 0;
-            const int key0 = (t0 + (int)(x - pos)) * kTileTokens;
-            if (!hidden) {
-                const uint8_t* tile = my_ring + stage * Cfg::TILE;
-                // ---- scores
-                uint32_t ka[W], kb[W];
-                const uint8_t* kr = tile + g * (D / 2) + t * (D / 8);
+        // KT tiles; MASKED: some key of theirs is not there for some column
+        auto work = [&](const uint8_t* tile, const int key0, const int hidden, auto masked) {
+            constexpr bool MASKED = decltype(masked)::value;
+            constexpr int KT = Cfg::KT;
+            // ---- scores
+            __half2 kp[KT][2][GR];  // this lane's two keys' pairs
+            uint32_t ka[KT][W], kb[KT][W];
 #pragma unroll
-                for (int w = 0; w < W; w += (W < 4 ? W : 4)) {
-                    if constexpr (W == 2) {
-                        const uint2 a = *reinterpret_cast<const uint2*>(kr), c = *reinterpret_cast<const uint2*>(kr + 4 * D);
-                        ka[0] = a.x; ka[1] = a.y; kb[0] = c.x; kb[1] = c.y;
-                    } else {
-                        const uint4 a = *reinterpret_cast<const uint4*>(kr + 4 * w), c = *reinterpret_cast<const uint4*>(kr + 4 * D + 4 * w);
-                        ka[w] = a.x; ka[w + 1] = a.y; ka[w + 2] = a.z; ka[w + 3] = a.w;
-                        kb[w] = c.x; kb[w + 1] = c.y; kb[w + 2] = c.z; kb[w + 3] = c.w;
-                    }
-                }
-                float sc[NT][4];
+            for (int k = 0; k < KT; ++k) {
+                const uint8_t* kr = tile + k * Cfg::TILE + g * (D / 2) + t * (D / 8);
+                load_words<W>(kr, ka[k]);
+                load_words<W>(kr + 4 * D, kb[k]);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int r = 0; r < 2; ++r) load_pairs<GR>(tile + k * Cfg::TILE + pair_at(D, 0, g + 8 * r, 0), kp[k][r]);
+            }
+            float sc[KT][NT][4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) sc[nt][e] = 0.f;
+            for (int gr = 0; gr < GR; ++gr) {
+                float d[KT][NT][4];
 #pragma unroll
-                for (int gr = 0; gr < GR; ++gr) {
-                    float d[NT][4];
+                for (int k = 0; k < KT; ++k)
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) d[nt][e] = 0.f;
+                        for (int e = 0; e < 4; ++e) d[k][nt][e] = 0.f;
 #pragma unroll
-                    for (int w = 2 * gr; w < 2 * gr + 2; ++w)
+                for (int w = 2 * gr; w < 2 * gr + 2; ++w)
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const uint32_t ua = ka[w] >> (8 * h), ub = kb[w] >> (8 * h);
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int k = 0; k < KT; ++k) {
+                            const uint32_t ua = ka[k][w] >> (8 * h), ub = kb[k][w] >> (8 * h);
                             const uint32_t a0 = ua & 0x000f000fu, a1 = ub & 0x000f000fu, a2 = ua & 0x00f000f0u, a3 = ub & 0x00f000f0u;
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                                for (int pl = 0; pl < PL; ++pl) ptx::mma_bf16_16816(d[nt], a0, a1, a2, a3, qf[nt][pl][w][2 * h], qf[nt][pl][w][2 * h + 1]);
+                                for (int pl = 0; pl < PL; ++pl) ptx::mma_bf16_16816(d[k][nt], a0, a1, a2, a3, qf[nt][pl][w][2 * h], qf[nt][pl][w][2 * h + 1]);
                         }
-                    const float2 pa = __half22float2(*reinterpret_cast<const __half2*>(tile + pair_at(D, 0, g, gr)));
-                    const float2 pb = __half22float2(*reinterpret_cast<const __half2*>(tile + pair_at(D, 0, g + 8, gr)));
-                    const float sa = pa.x * code_mul, sb = pb.x * code_mul;
+#pragma unroll
+                for (int k = 0; k < KT; ++k) {
+                    const float2 pa = __half22float2(kp[k][0][gr]), pb = __half22float2(kp[k][1][gr]);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            sc[nt][c] = fmaf(sa, d[nt][c], fmaf(pa.y, qsum[nt][gr][c], sc[nt][c]));
-                            sc[nt][2 + c] = fmaf(sb, d[nt][2 + c], fmaf(pb.y, qsum[nt][gr][c], sc[nt][2 + c]));
+                        for (int r = 0; r < 4; r += 2) {
+                            const float least = r ? pb.y : pa.y, scale = r ? pb.x : pa.x;
+#pragma unroll
+                            for (int c = 0; c < 2; ++c) {  // (packed pairs would need both factors twice)
+                                const float low = gr == 0 ? least * qsum[nt][gr][c] : fmaf(least, qsum[nt][gr][c], sc[k][nt][r + c]);
+                                sc[k][nt][r + c] = fmaf(scale, d[k][nt][r + c], low);
+                            }
                         }
                 }
-                const bool masked = key0 + kTileTokens > least_limit;  // uniform over the warp
-                if (masked) {
+            }
+            auto visible = [&](int k, int nt, int e) {
+                return ((hidden >> k) & 1) == 0 && key0 + k * kTileTokens + g + (e & 2) * 4 < limit[nt][e & 1];
+            };
+            if (MASKED) {
+#pragma unroll
+                for (int k = 0; k < KT; ++k)
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            if (key0 + g + (e & 2) * 4 >= limit[nt][e & 1]) sc[nt][e] = -INFINITY;
+                            if (!visible(k, nt, e)) sc[k][nt][e] = -INFINITY;
+            }
+            // ---- softmax
+            float mx[NT][2];
+            bool grow = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    mx[nt][c] = fmaxf(sc[0][nt][c], sc[0][nt][2 + c]);
+                    if (KT == 2) mx[nt][c] = ptx::fmax3(mx[nt][c], sc[KT - 1][nt][c], sc[KT - 1][nt][2 + c]);
+                    grow = grow || mx[nt][c] > bar[nt][c];
                 }
-                // ---- softmax
-                bool grow = false;
+            if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) grow = grow || fmaxf(sc[nt][c], sc[nt][2 + c]) > m[nt][c] + 8.f;
-                if (__any_sync(0xffffffffu, grow)) {
+                    for (int c = 0; c < 2; ++c) {
+                        float top = mx[nt][c];
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                        const float to = fmaxf(m[nt][c], top);
+                        const float alpha = to == -INFINITY ? 1.f : ptx::ex2_approx((m[nt][c] - to) * to_log2);
+                        m[nt][c] = to;
+                        bar[nt][c] = to + step;
+                        use[nt][c] = to == -INFINITY ? 64.f : fmaf(-to, to_log2, 64.f);
+                        l[nt][c] *= alpha;
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
+                        for (int gr = 0; gr < GR; ++gr) low[nt][gr][c] *= alpha;
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            float mx = fmaxf(sc[nt][c], sc[nt][2 + c]);
-                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                            const float to = fmaxf(m[nt][c], mx);
-                            const float alpha = to == -INFINITY ? 1.f : ptx::ex2_approx(m[nt][c] - to);
-                            m[nt][c] = to;
-                            l[nt][c] *= alpha;
-#pragma unroll
-                            for (int gr = 0; gr < GR; ++gr) low[nt][gr][c] *= alpha;
-#pragma unroll
-                            for (int i = 0; i < 2 * W; ++i) {
-                                acc[nt][i][c] *= alpha;
-                                acc[nt][i][2 + c] *= alpha;
-                            }
+                        for (int i = 0; i < 2 * W; ++i) {
+                            acc[nt][i][c] *= alpha;
+                            acc[nt][i][2 + c] *= alpha;
                         }
-                }
-                float pr[NT][4];
+                    }
+            }
+            float pr[KT][NT][4];
+#pragma unroll
+            for (int k = 0; k < KT; ++k)
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float mc = m[nt][e & 1];
-                        pr[nt][e] = ptx::ex2_approx(sc[nt][e] - (mc == -INFINITY ? 0.f : mc));
-                        l[nt][e & 1] += pr[nt][e];
+                    for (int r = 0; r < 4; r += 2) {
+                        float x0, x1;
+                        ptx::fma2(x0, x1, sc[k][nt][r], sc[k][nt][r + 1], to_log2, to_log2, use[nt][0], use[nt][1]);
+                        pr[k][nt][r] = ptx::ex2_approx(x0);
+                        pr[k][nt][r + 1] = ptx::ex2_approx(x1);
+                        ptx::add2(l[nt][0], l[nt][1], l[nt][0], l[nt][1], pr[k][nt][r], pr[k][nt][r + 1]);
                     }
-                // ---- output
-                uint32_t v[4][GR];
+            // ---- output
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const uint8_t* vr = tile + 8 * D + (4 * c + t) * (D / 2) + (g ^ (2 * t)) * (D / 16);
-                    if constexpr (GR == 1) {
-                        v[c][0] = *reinterpret_cast<const uint32_t*>(vr);
-                    } else if constexpr (GR == 2) {
-                        const uint2 u = *reinterpret_cast<const uint2*>(vr);
-                        v[c][0] = u.x; v[c][1] = u.y;
-                    } else {
-                        const uint4 u = *reinterpret_cast<const uint4*>(vr);
-                        v[c][0] = u.x; v[c][1] = u.y; v[c][2] = u.z; v[c][3] = u.w;
-                    }
-                }
+            for (int k = 0; k < KT; ++k) {
+                uint32_t v[4][GR];
+                __half2 vp[2][GR];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) load_words<GR>(tile + k * Cfg::TILE + 8 * D + (4 * c + t) * (D / 2) + (g ^ (2 * t)) * (D / 16), v[c]);
+#pragma unroll
+                for (int r = 0; r < 2; ++r) load_pairs<GR>(tile + k * Cfg::TILE + pair_at(D, 1, g + 8 * r, 0), vp[r]);
 #pragma unroll
                 for (int gr = 0; gr < GR; ++gr) {
-                    const float2 pa = __half22float2(*reinterpret_cast<const __half2*>(tile + pair_at(D, 1, g, gr)));
-                    const float2 pb = __half22float2(*reinterpret_cast<const __half2*>(tile + pair_at(D, 1, g + 8, gr)));
-                    const float sa = pa.x * 0x1p64f, sb = pb.x * 0x1p64f;
+                    const float2 pa = __half22float2(vp[0][gr]), pb = __half22float2(vp[1][gr]);
                     uint32_t f[NT][2][2];  // [.][plane][keys 0-7, 8-15]
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        float w[4], y[4];
+                        float w[4];
+                        if (MASKED) {  // (a hidden key's scale may be anything)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            w[e] = pr[nt][e] * ((e & 2) ? sb : sa);
-                            y[e] = pr[nt][e] * ((e & 2) ? pb.y : pa.y);
+                            for (int e = 0; e < 4; ++e) {
+                                const bool on = visible(k, nt, e);
+                                w[e] = on ? pr[k][nt][e] * ((e & 2) ? pb.x : pa.x) : 0.f;
+                                low[nt][gr][e & 1] += on ? pr[k][nt][e] * ((e & 2) ? pb.y : pa.y) : 0.f;
+                            }
+                        } else {
+#pragma unroll
+                            for (int r = 0; r < 4; r += 2) {
+                                const float least = r ? pb.y : pa.y, scale = r ? pb.x : pa.x;
+#pragma unroll
+                                for (int c = 0; c < 2; ++c) {
+                                    w[r + c] = pr[k][nt][r + c] * scale;
+                                    low[nt][gr][c] = fmaf(pr[k][nt][r + c], least, low[nt][gr][c]);
+                                }
+                            }
                         }
-                        if (masked) {  // (a hidden key's scale may be anything)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                if (key0 + g + (e & 2) * 4 >= limit[nt][e & 1]) w[e] = y[e] = 0.f;
-                        }
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) low[nt][gr][c] += y[c] + y[2 + c];
 #pragma unroll
                         for (int r = 0; r < 2; ++r) {
                             const uint32_t top = ptx::pack2<__nv_bfloat16>(w[2 * r], w[2 * r + 1]);
@@ -522,9 +588,25 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
                     }
                 }
             }
+        };
+        const int seg_at = (int)(pos - start);  // of the range
+        for (int at = warp + kWarps * done - seg_at; at < seg; at += kWarps) {
+            if (!__all_sync(0xffffffffu, wait_stage(&my_bars[stage], phase, abort_flag))) { ok = false; break; }
+            const int hidden = my_hidden[stage];
+#pragma unroll 1
+            for (int k0 = 0; k0 < kBlockTiles; k0 += Cfg::KT) {
+                const int key0 = (t0 + at) * kBlockKeys + k0 * kTileTokens;
+                const uint8_t* tile = my_ring + stage * Cfg::STAGE + k0 * Cfg::TILE;
+                if (key0 + Cfg::KT * kTileTokens > least_limit || (hidden >> k0) != 0) work(tile, key0, hidden >> k0, std::true_type{});  // uniform over the warp
+                else work(tile, key0, 0, std::false_type{});
+            }
             __syncwarp();  // every lane has read the stage
-            issue(done + kStages);
+            issue(done + Cfg::STAGES, stage);
             ++done;
+            if (++stage == Cfg::STAGES) {
+                stage = 0;
+                phase ^= 1u;
+            }
         }
         if (!ok) break;
 
@@ -539,17 +621,17 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
 #pragma unroll
                     for (int gr = 0; gr < GR; ++gr) low[nt][gr][c] += __shfl_xor_sync(0xffffffffu, low[nt][gr][c], o);
                 }
-                if (g == 0) ml_s[warp * Cfg::COLS + nt * 8 + 2 * t + c] = make_float2(m[nt][c], l[nt][c]);
+                if (g == 0) ml_s[warp * Cfg::COLS + nt * 8 + 2 * t + c] = make_float2(m[nt][c] * to_log2, l[nt][c]);
 #pragma unroll
                 for (int i = 0; i < 2 * W; ++i) {  // block i: channels 64 (i / 4) + 8 g + 2 (i % 4) + {0, 1}
                     const float base = low[nt][i / 4][c];
-                    const float2 y = make_float2(fmaf(acc[nt][i][c], 0x1p69f, base), fmaf(acc[nt][i][2 + c], 0x1p65f, base));
+                    const float2 y = make_float2(fmaf(acc[nt][i][c] * 0x1p69f, 0x1p64f, base), fmaf(acc[nt][i][2 + c] * 0x1p65f, 0x1p64f, base));
                     *reinterpret_cast<float2*>(o_s + (warp * Cfg::COLS + nt * 8 + 2 * t + c) * Cfg::O_STRIDE + 64 * (i / 4) + 8 * g + 2 * (i & 3)) = y;
                 }
             }
         __syncthreads();
         if (*abort_flag) { ok = false; break; }
-        const bool whole = seg == n_tiles;
+        const bool whole = seg == n_blocks;
         const int64_t slot = 2 * (int64_t)blockIdx.x + (t0 == 0 ? 1 : 0);
         const int cols = min(Cfg::COLS, count * p.group - ct * Cfg::COLS);
         for (int i = tid; i < cols * (D / 8); i += kWarps * 32) {
@@ -582,7 +664,7 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
             }
         }
         if (!whole && t0 == 0 && tid == 0) {  // the unit goes on in the next ranges
-            const int64_t unit_end = pos + n_tiles;
+            const int64_t unit_end = pos + n_blocks;
             int parts = 1;
             while (total * ((int64_t)blockIdx.x + parts) / ranges < unit_end) ++parts;
             *desc = {parts, first_s[b], count, kvh, ct, {0, 0, 0}};
@@ -687,7 +769,7 @@ int attend_split(const AttendParams& whole, int64_t D, int64_t max_q, void* work
         else sp.a.row0 = at;
         sp.parts = static_cast<float*>(workspace);
         sp.split = cut(max_len);
-        sp.min_tiles = 8;
+        sp.min_blocks = 8;
         sp.first_rows = at == 0;
         sp.last_rows = at + kMaxBatch >= whole.batch;
         int rc;
@@ -735,6 +817,9 @@ extern "C" int xg_kv4_attention(const void* q, const void* cache, int64_t pages,
         return fail(XG_ERR_INVALID_ARG, "xg_kv4_attention: bad extents");
     if (q_heads > 65535 || batch > 0x7fffff || tokens > 0x7fffffff || table_pages > 0x7ffffff) return fail(XG_ERR_TOO_LARGE, "xg_kv4_attention: extents");
     if (table_pages * page_size > 0x7fffff00LL) return fail(XG_ERR_TOO_LARGE, "xg_kv4_attention: more than 2^31 tokens per sequence");
+    // a range of tiles is counted in 32 bits (2^38 tiles are 300 TB of cache read, or some minutes)
+    if (tokens > 0 && kv_heads * (tokens * (q_heads / kv_heads) / 8 + batch + 1) > (1LL << 38) / (table_pages * (page_size / 16) + 1))
+        return fail(XG_ERR_TOO_LARGE, "xg_kv4_attention: too many rows and keys");
     if (tokens == 0) return XG_OK;
     if (!q || !out || (batch > 0 && (!kv_lens || (table_pages > 0 && !page_table)))) return fail(XG_ERR_INVALID_ARG, "xg_kv4_attention: null pointer");
     if (!aligned16(out)) return fail(XG_ERR_INVALID_ARG, "xg_kv4_attention: the result must be 16-byte aligned");
