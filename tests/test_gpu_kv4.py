@@ -221,6 +221,14 @@ ATTEND = [  # d, kv heads, group, page, lens, new tokens (None: one each, withou
     (256, 2, 1, 16, [90, 40], [4, 6]),
     (128, 1, 1, 16, [2, 3], [4, 5]),  # more rows than tokens: the first ones see nothing
     (128, 3, 2, 64, [9000, 8999], None),
+    # many new tokens, alone and beside few
+    (128, 2, 4, 16, [300, 100, 17, 0, 64, 70], [100, 40, 17, 0, 3, 64]),
+    (64, 1, 1, 64, [513, 130], [513, 129]),
+    (128, 1, 8, 32, [1500], [300]),
+    (128, 4, 3, 16, [257, 77, 500], [86, 77, 85]),
+    (64, 2, 5, 128, [3000, 64], [40, 64]),
+    (128, 1, 1, 16, [70, 0, 100], [90, 66, 130]),
+    (256, 1, 2, 32, [150], [150]),
 ]
 
 
@@ -239,7 +247,7 @@ def test_attention(cuda_device, d, heads, group, page, lens, new, dtype):
     at = None if starts is None else torch.tensor(starts, device=cuda_device)
     got = ops.kv4_attention(q, cache, table, torch.tensor(lens, device=cuda_device), at, max(new or [1]), d ** -0.5)
     assert got.dtype == dtype and got.is_contiguous()
-    _check_attention(got, _reference(q, cache, table, lens, starts, d ** -0.5), "attention")
+    _check_attention(got, _reference(q, cache, table, lens, starts, d ** -0.5), "attention", halves=max(new or [1]) > 8)
     if starts is not None:
         assert not got[starts[-1]:].any()
     assert lib.tc_status() == 0
@@ -287,6 +295,34 @@ def test_attention_leaves_alone_what_is_not_there(cuda_device):
     assert not ops.kv4_attention(q, cache, table[:, :0], n, None, 1, 0.1).any()
     assert not ops.kv4_attention(q, cache[:0], table, n, None, 1, 0.1).any()
     assert ops.kv4_attention(q[:0], cache, table[:0], n[:0], None, 1, 0.1).shape == (0, 4, 128)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_attention_of_many_new_tokens(cuda_device, dtype):
+    """Holes, NaN behind the end, scores of hundreds, a negative and a zero scale, rows of q of any size and alignment."""
+    from xpu_graph_b200 import lib, ops
+
+    lens, starts = [333, 200], [0, 200, 350]
+    cache = _filled(20, 2, 32, 128, cuda_device, scale=3.0)
+    table = torch.cat((_table([352, 224], 32, 20, cuda_device), torch.full((2, 3), -7, device=cuda_device)), 1)
+    nan = torch.full((32, 2, 128), math.nan, device=cuda_device)
+    for b, n in enumerate(lens):
+        j = torch.arange(n, -(-n // 32) * 32, device=cuda_device)
+        ops.kv4_append(cache, nan[:len(j)], nan[:len(j)], table[b, j // 32] * 32 + j % 32)
+    table[0, 3] = 20
+    table[0, 10 - 1] = -1
+    table[1, 0] = 1 << 33
+    g = torch.Generator().manual_seed(1)
+    q = torch.randn(350, 6 * 128 + 3, generator=g).to(dtype)[:, 3:].unflatten(1, (6, 128)).to(cuda_device)
+    q = q * torch.tensor([1e-3, 1.0, 100.0]).to(dtype).to(cuda_device)[torch.arange(350, device=cuda_device) % 3][:, None, None]
+    q[5] = 0
+    n, at = torch.tensor(lens, device=cuda_device), torch.tensor(starts, device=cuda_device)
+    for scale in (0.08, -0.05, 0.0):
+        got = ops.kv4_attention(q, cache, table, n, at, 200, scale)
+        assert torch.isfinite(got).all()
+        _check_attention(got, _reference(q, cache, table, lens, starts, scale), f"scale {scale}", halves=True)
+        assert torch.equal(got, ops.kv4_attention(q, cache, table, n, at, 200, scale))
+    assert lib.tc_status() == 0
 
 
 def test_attention_is_repeatable_and_any_hint_will_do(cuda_device):

@@ -38,6 +38,7 @@ SOURCES = [
     "qk_norm_rope.cu",
     "kv4_cache.cu",
     "kv4_attention.cu",
+    "kv4_prefill.cu",
     "sum3d.cu",
     "rowsum_cat.cu",
 ]

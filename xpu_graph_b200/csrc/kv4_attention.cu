@@ -1,10 +1,7 @@
 // Attention over the 4-bit cache: out = softmax(q k^T * scale) v for the newest tokens of every sequence. Query token i of the n_b new
 // ones of sequence b stands at position len_b - n_b + i and sees the keys up to its own. Heads are grouped: query head h reads kv
 // head h / (Hq / Hkv). fp32 scores, softmax and sums.
-#include "kv4_tile.cuh"
-#include "sm100_ptx.cuh"
-
-#include <type_traits>
+#include "kv4_attend.cuh"
 
 namespace xg {
 
@@ -14,53 +11,6 @@ __device__ unsigned int g_kv4_status[4];
 namespace {
 
 using namespace kv4;
-constexpr float kLog2e = 1.4426950408889634f;
-
-struct AttendParams {
-    Cache cache;
-    const void* q;
-    void* out;  // [tokens, Hq, D]
-    const int64_t* table;
-    const int64_t* lens;
-    const int64_t* starts;  // null: one new token per sequence
-    int64_t q_st, q_sh, table_stride;
-    int64_t tokens;
-    int batch, heads, group, table_pages;
-    int row0;  // without starts: the row of the first sequence
-    float scale;
-};
-
-__device__ __forceinline__ int64_t clamp64(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : (v > hi ? hi : v); }
-
-// Rows [first, first + count) of q that belong to sequence b, and its number of cached tokens.
-struct Sequence {
-    int64_t first, len;
-    int count;
-};
-__device__ __forceinline__ Sequence sequence(const AttendParams& p, int b) {
-    Sequence s;
-    int64_t end;
-    if (p.starts) {
-        s.first = clamp64(p.starts[b], 0, p.tokens);
-        end = clamp64(p.starts[b + 1], s.first, p.tokens);
-    } else {
-        s.first = p.row0 + b;
-        end = s.first + 1;
-    }
-    s.count = (int)(end - s.first);
-    s.len = clamp64(p.lens[b], 0, (int64_t)p.table_pages * p.cache.tiles * kTileTokens);
-    return s;
-}
-
-// 8 channels of a finished row; a row that saw no key is zeros.
-template <typename T>
-__device__ __forceinline__ void store_row8(T* out, const float (&o)[8], float sum) {
-    const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
-    Vec16<T> y;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) y.v[e] = Cvt<T>::from_f(o[e] * inv);
-    st16(out, y);
-}
 
 // ---------------------------------------------------------------------------------------
 // Few query rows per sequence: the cache streamed once
@@ -108,6 +58,7 @@ struct SplitParams {
     float* parts;  // [2 * gridDim.x][COLS][D] sums, then [2 * gridDim.x][COLS] (maximum, sum) pairs, then a PartDesc per CTA
     int split;         // 0: a unit stays in one CTA
     int64_t min_blocks; // of a range
+    int most_cols;       // sequences with more columns are left alone
     int first_rows, last_rows;  // this launch zeroes the rows before the first / behind the last sequence
 };
 
@@ -122,49 +73,8 @@ struct Planes {
     static constexpr int N = std::is_same<T, __nv_bfloat16>::value ? 1 : 2;
 };
 
-template <typename T>
-__device__ __forceinline__ uint4 load_q8(const T* p, bool vec) {  // 8 elements
-    if (vec) return *reinterpret_cast<const uint4*>(p);
-    const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = (uint32_t)h[2 * i] | ((uint32_t)h[2 * i + 1] << 16);
-    return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
 __device__ __forceinline__ float bf16_lo(uint32_t x) { return __uint_as_float(x << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
-
-// N 32-bit words at once
-template <int N>
-__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&out)[N]) {
-    if constexpr (N == 1) {
-        out[0] = *reinterpret_cast<const uint32_t*>(p);
-    } else if constexpr (N == 2) {
-        const uint2 u = *reinterpret_cast<const uint2*>(p);
-        out[0] = u.x; out[1] = u.y;
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i += 4) {
-            const uint4 u = *reinterpret_cast<const uint4*>(p + 4 * i);
-            out[i] = u.x; out[i + 1] = u.y; out[i + 2] = u.z; out[i + 3] = u.w;
-        }
-    }
-}
-// N (scale, least) pairs at once
-template <int N>
-__device__ __forceinline__ void load_pairs(const uint8_t* p, __half2 (&out)[N]) {
-    uint32_t u[N];
-    load_words<N>(p, u);
-#pragma unroll
-    for (int i = 0; i < N; ++i) out[i] = *reinterpret_cast<const __half2*>(&u[i]);
-}
-
-// The usual case is one question; what waits longer does so outside the loop's code.
-__device__ __noinline__ bool wait_longer(uint64_t* bar, uint32_t phase, volatile int* abort_flag) { return ptx::mbar_wait_bounded(bar, phase, abort_flag); }
-__device__ __forceinline__ bool wait_stage(uint64_t* bar, uint32_t phase, volatile int* abort_flag) {
-    return ptx::mbar_try_wait(bar, phase) || wait_longer(bar, phase, abort_flag);
-}
 
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_split_kernel(const SplitParams sp) {
@@ -205,8 +115,9 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
             const Sequence s = sequence(p, b);
             first_s[b] = (int)s.first;
             count_s[b] = s.count;
-            len_s[b] = (int)s.len;
-            w = (int64_t)kv_heads * col_tiles(s.count) * ((s.len + kBlockKeys - 1) / kBlockKeys);
+            const int len = s.count * p.group > sp.most_cols ? -1 : (int)s.len;
+            len_s[b] = len;
+            w = (int64_t)kv_heads * col_tiles(s.count) * ((max(len, 0) + kBlockKeys - 1) / kBlockKeys);
         }
         int64_t inc = w;
 #pragma unroll
@@ -294,10 +205,7 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
         for (int k = 0; k < kBlockTiles; ++k) {
             const int tile = (int)(off - unit * n) * kBlockTiles + k;
             if (tile * kTileTokens >= len_s[b]) break;
-            const int page = tile / p.cache.tiles;
-            const int64_t id = p.table[(int64_t)b * p.table_stride + page];
-            if (id >= 0 && id < p.cache.pages)
-                addr[k] = reinterpret_cast<int64_t>(p.cache.base + id * p.cache.page_stride + ((int64_t)kvh * p.cache.tiles + (tile - page * p.cache.tiles)) * Cfg::TILE);
+            addr[k] = tile_of_token(p, b, kvh, tile, Cfg::TILE);
         }
     };
     auto issue = [&](int i, int stage) {
@@ -435,12 +343,6 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
             for (int gr = 0; gr < GR; ++gr) {
                 float d[KT][NT][4];
 #pragma unroll
-                for (int k = 0; k < KT; ++k)
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) d[k][nt][e] = 0.f;
-#pragma unroll
                 for (int w = 2 * gr; w < 2 * gr + 2; ++w)
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
@@ -451,7 +353,10 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                                for (int pl = 0; pl < PL; ++pl) ptx::mma_bf16_16816(d[k][nt], a0, a1, a2, a3, qf[nt][pl][w][2 * h], qf[nt][pl][w][2 * h + 1]);
+                                for (int pl = 0; pl < PL; ++pl) {
+                                    if (w == 2 * gr && h == 0 && pl == 0) ptx::mma_bf16_16816_first(d[k][nt], a0, a1, a2, a3, qf[nt][pl][w][0], qf[nt][pl][w][1]);
+                                    else ptx::mma_bf16_16816(d[k][nt], a0, a1, a2, a3, qf[nt][pl][w][2 * h], qf[nt][pl][w][2 * h + 1]);
+                                }
                         }
 #pragma unroll
                 for (int k = 0; k < KT; ++k) {
@@ -755,8 +660,10 @@ int64_t split_workspace(int64_t D, int64_t max_q, int64_t group, int64_t max_len
     return 2 * ctas * cols * (D + 2) * 4 + ctas * (int64_t)sizeof(PartDesc);
 }
 
+constexpr int kMostStreamed = 64;
+
 template <typename T>
-int attend_split(const AttendParams& whole, int64_t D, int64_t max_q, void* workspace, cudaStream_t st) {
+int attend_split(const AttendParams& whole, int64_t D, int64_t max_q, int most_cols, void* workspace, cudaStream_t st) {
     const int64_t max_len = (int64_t)whole.table_pages * whole.cache.tiles * kTileTokens;
     const int cols = columns(D, max_q, whole.group);
     for (int at = 0; at == 0 || at < whole.batch; at += kMaxBatch) {
@@ -770,6 +677,7 @@ int attend_split(const AttendParams& whole, int64_t D, int64_t max_q, void* work
         sp.parts = static_cast<float*>(workspace);
         sp.split = cut(max_len);
         sp.min_blocks = 8;
+        sp.most_cols = most_cols;
         sp.first_rows = at == 0;
         sp.last_rows = at + kMaxBatch >= whole.batch;
         int rc;
@@ -790,6 +698,9 @@ int read_kv4_status(unsigned int* host_out, int reset) {
         return fail(XG_ERR_DEVICE, "xg_tc_status: cannot read device status");
     }
     *host_out = v[0];
+    unsigned int more = 0;
+    if (const int rc = read_kv4_prefill_status(&more, reset)) return rc;
+    *host_out |= more << 1;
     if (reset && v[0] != 0) {
         unsigned int z[4] = {0, 0, 0, 0};
         cudaMemcpyToSymbol(g_kv4_status, z, sizeof(z));
@@ -833,5 +744,9 @@ extern "C" int xg_kv4_attention(const void* q, const void* cache, int64_t pages,
     if (workspace_bytes < need || (need > 0 && (!workspace || !aligned16(workspace))))
         return fail(XG_ERR_INVALID_ARG, "xg_kv4_attention: needs %lld bytes of 16-byte aligned workspace", (long long)need);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    return dtype == XG_BF16 ? attend_split<__nv_bfloat16>(p, D, max_q, workspace, st) : attend_split<__half>(p, D, max_q, workspace, st);
+    // Sequences with many columns go to the tensor-memory kernel, where there may be any; the others to the streaming one.
+    const bool tiles = D != 256 && batch > 0 && max_q * p.group > kMostStreamed;
+    const int most = tiles ? kMostStreamed : 0x7fffffff;
+    const int rc = dtype == XG_BF16 ? attend_split<__nv_bfloat16>(p, D, max_q, most, workspace, st) : attend_split<__half>(p, D, max_q, most, workspace, st);
+    return rc != XG_OK || !tiles ? rc : attend_prefill(p, D, dtype, most, st);
 }

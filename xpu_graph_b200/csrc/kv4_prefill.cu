@@ -1,0 +1,533 @@
+// Attention of many new tokens over the 4-bit cache: flash attention on tcgen05 with keys and values unpacked on the way in.
+//
+// A CTA owns 256 rows of one kv head - rows are the (new token, head of the group) pairs in token order, so that all heads of a group
+// share the unpacked keys - as two 128-row tiles. Per block of 64 keys: four warps unpack K and V, one 16-key tile each, from a ring of
+// bulk copies into fp16 operand tiles (128-byte swizzle, the layout a tensor map would leave); one thread issues S = Q K^T for both
+// tiles into double-buffered tensor memory, then O += P V with P read from tensor memory; eight warps (a row per thread) turn
+// scores into probabilities in place, as flash_tc_kernel (sdpa.cu) does, with the maximum lagging by up to 2^8.
+//
+// Everything that meets in a product is fp16: codes are exact there, code * scale + least is rounded once (2^-12 relative), as are
+// probabilities; fp16 queries stay as they are and bf16 ones too, after a power of two per row has been taken out (it returns in the
+// row's exponent factor). Sums are fp32 in tensor memory and registers.
+//
+// What bounds it: unpacking 64 keys (2 operations per code) and 256 x 64 exponentials run beside 1024 cycles of products per block.
+#include "kv4_attend.cuh"
+
+namespace xg {
+
+__device__ unsigned int g_kv4_prefill_status[4];
+
+namespace {
+
+using namespace kv4;
+
+constexpr int PM = 128;  // rows per tile
+constexpr int PN = 64;   // keys per block
+constexpr int kUnpackWarps = 4, kRing = 4;
+constexpr int kPrefillThreads = (kUnpackWarps + 1 + 8) * 32;
+constexpr float kLag = 8.0f;  // log2 units
+
+template <int D>
+struct PreCfg {
+    static constexpr int Q_BYTES = PM * D * 2;
+    static constexpr int KV_BYTES = PN * D * 2;
+    static constexpr int TILE = tile_bytes(D);
+    static constexpr int RING = kUnpackWarps * kRing * TILE;
+    static constexpr int SMEM = 2 * Q_BYTES + 4 * KV_BYTES + RING + 512;
+};
+
+struct Unit {
+    int on, b, kvh, rt;  // rt: which 256 rows
+    int first, count, len;
+};
+
+// 8 codes as fp16 values, in channel order
+__device__ __forceinline__ uint4 unpack8(uint32_t w, __half2 scale, __half2 least) {
+    uint32_t out[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        // byte k in both halves; its low code becomes 1024 + n in the low half, its high code 64 + n in the high half
+        const uint32_t y = (__byte_perm(w, 0, 0x4040 + k * 0x0101) & 0x00f0000fu) | 0x54006400u;
+        const __half2 n = __hsub2(*reinterpret_cast<const __half2*>(&y), __halves2half2(__ushort_as_half(0x6400), __ushort_as_half(0x5400)));
+        const __half2 v = __hfma2(n, scale, least);
+        out[k] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+    return make_uint4(out[0], out[1], out[2], out[3]);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const AttendParams p, int beyond) {
+    using Cfg = PreCfg<D>;
+    constexpr int W = D / 32, GR = D / 64;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint8_t* q_s = smem;                          // [2][Q_BYTES]; at the end the output rows on their way out
+    uint8_t* k_s = q_s + 2 * Cfg::Q_BYTES;        // [2][KV_BYTES]
+    uint8_t* v_s = k_s + 2 * Cfg::KV_BYTES;       // [2][KV_BYTES]
+    uint8_t* ring = v_s + 2 * Cfg::KV_BYTES;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(ring + Cfg::RING);
+    uint64_t* q_full = bars;          // [tile]
+    uint64_t* k_full = bars + 2;      // [buffer]
+    uint64_t* k_empty = bars + 4;
+    uint64_t* v_full = bars + 6;
+    uint64_t* v_empty = bars + 8;
+    uint64_t* s_full = bars + 10;     // [tile][buffer]
+    uint64_t* p_full = bars + 14;     // [tile][buffer]
+    uint64_t* pv_full = bars + 18;    // [tile]
+    uint64_t* o_full = bars + 20;     // [tile]
+    uint64_t* drain_bar = bars + 22;
+    uint64_t* ring_full = bars + 23;  // [warp][stage]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 23 + kUnpackWarps * kRing);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile int* holes = abort_flag + 1;                    // [4][warp]: a block's tiles that are not in the cache
+    volatile int* ring_hole = holes + 4 * kUnpackWarps;      // [warp][stage]
+    Unit* unit = reinterpret_cast<Unit*>(const_cast<int*>(ring_hole + kUnpackWarps * kRing));
+    static_assert(23 * 8 + kUnpackWarps * kRing * 8 + 8 + (4 * kUnpackWarps + kUnpackWarps * kRing) * 4 + sizeof(Unit) <= 512, "barriers");
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if ((ptx::smem_u32(smem) & 1023u) != 0) {  // uniform over the CTA: the swizzled tiles need this alignment
+        pdl_sync();
+        if (threadIdx.x == 0) atomicOr(&g_kv4_prefill_status[0], 4u);
+        return;
+    }
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            ptx::mbar_init(&q_full[i], PM);
+            ptx::mbar_init(&k_full[i], kUnpackWarps);
+            ptx::mbar_init(&k_empty[i], 1);
+            ptx::mbar_init(&v_full[i], kUnpackWarps);
+            ptx::mbar_init(&v_empty[i], 1);
+            ptx::mbar_init(&pv_full[i], 1);
+            ptx::mbar_init(&o_full[i], 1);
+        }
+        for (int i = 0; i < 4; ++i) {
+            ptx::mbar_init(&s_full[i], 1);
+            ptx::mbar_init(&p_full[i], PM);
+        }
+        ptx::mbar_init(drain_bar, 1);
+        for (int i = 0; i < kUnpackWarps * kRing; ++i) ptx::mbar_init(&ring_full[i], 1);
+        *abort_flag = 0;
+        ptx::fence_mbar_init();
+        ptx::fence_proxy_async();
+    }
+    if (warp == kUnpackWarps) ptx::tmem_alloc(tmem_slot, 512);
+    pdl_sync();
+    if (warp == 0) {  // which rows are this CTA's: the sequences' units one after the other, the last rows (most keys) first
+        int base = 0;
+        Unit u = {};
+        for (int b0 = 0; b0 < p.batch; b0 += 32) {
+            const int b = b0 + lane;
+            Sequence s = {};
+            int w = 0;
+            if (b < p.batch) {
+                s = sequence(p, b);
+                if (s.count * p.group > beyond) w = (s.count * p.group + 2 * PM - 1) / (2 * PM) * p.cache.heads;
+            }
+            int inc = w;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += v;
+            }
+            const int at = (int)blockIdx.x - base;
+            if (at >= inc - w && at < inc) {
+                const int off = at - (inc - w), tiles = w / p.cache.heads;
+                u = {1, b, off % p.cache.heads, tiles - 1 - off / p.cache.heads, (int)s.first, s.count, (int)s.len};
+                *unit = u;
+            }
+            if (__any_sync(0xffffffffu, u.on)) break;
+            base += __shfl_sync(0xffffffffu, inc, 31);
+        }
+        if (!__any_sync(0xffffffffu, u.on) && lane == 0) unit->on = 0;
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const Unit u = *unit;
+
+    const int rows = u.count * p.group;
+    // key blocks of a tile: up to what its last row sees
+    auto blocks_of = [&](int i) {
+        const int lo = u.rt * 2 * PM + i * PM;
+        if (!u.on || lo >= rows) return 0;
+        const int seen = u.len - u.count + (min(rows, lo + PM) - 1) / p.group + 1;
+        return seen > 0 ? (seen + PN - 1) / PN : 0;
+    };
+    const int nblk0 = blocks_of(0), nblk1 = blocks_of(1), nblk = max(nblk0, nblk1);
+
+    if (warp < kUnpackWarps) {
+        // ------------------------------ unpacking ---------------------------------
+        uint8_t* my_ring = ring + warp * (kRing * Cfg::TILE);
+        uint64_t* my_full = ring_full + warp * kRing;
+        volatile int* my_hole = ring_hole + warp * kRing;
+        int64_t addr = 0;
+        auto issue = [&](int j) {  // this warp's tile of block j
+            if (j >= nblk) return;
+            if ((j & 31) == 0) {
+                const int tile = (j + lane) * kUnpackWarps + warp;
+                addr = tile * kTileTokens < u.len ? tile_of_token(p, u.b, u.kvh, tile, Cfg::TILE) : 0;
+            }
+            const int64_t from = __shfl_sync(0xffffffffu, addr, j & 31);
+            const int stage = j % kRing;
+            if (lane == 0) {
+                my_hole[stage] = from == 0;
+                if (from != 0) {
+                    ptx::mbar_arrive_expect_tx(&my_full[stage], Cfg::TILE);
+                    ptx::bulk_load(my_ring + stage * Cfg::TILE, reinterpret_cast<const void*>(from), Cfg::TILE, &my_full[stage]);
+                } else {
+                    ptx::mbar_arrive(&my_full[stage]);
+                }
+            }
+        };
+        for (int j = 0; j < kRing; ++j) issue(j);
+        const __half2 zero = __half2half2(__ushort_as_half(0));
+        bool ok = true;
+        // keys: a lane takes chunk t of rows r and r + 8; the bits are dealt so that neither its reads nor its swizzled writes collide
+        const int kr = (lane & 1) | ((lane >> 3) & 1) << 1 | ((lane >> 1) & 1) << 2, kt = ((lane >> 4) & 1) | ((lane >> 2) & 1) << 1;
+        for (int j = 0; j < nblk; ++j) {
+            const int stage = j % kRing, buf = j & 1;
+            const uint32_t ph = (uint32_t)(j >> 1) & 1u;
+            if (!__all_sync(0xffffffffu, ptx::mbar_wait_bounded(&my_full[stage], (uint32_t)(j / kRing) & 1u, abort_flag))) { ok = false; break; }
+            const uint8_t* tile = my_ring + stage * Cfg::TILE;
+            const int hole = my_hole[stage];
+            const int there = hole ? 0 : u.len - (j * kUnpackWarps + warp) * kTileTokens;  // tokens of the tile that exist
+            if (!__all_sync(0xffffffffu, ptx::mbar_wait_bounded(&k_empty[buf], ph ^ 1u, abort_flag))) { ok = false; break; }
+            if (lane == 0) holes[(j & 3) * kUnpackWarps + warp] = hole;
+            {
+                const uint32_t base = ptx::smem_u32(k_s + buf * Cfg::KV_BYTES) + (uint32_t)(warp * kTileTokens * 128);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int r = kr + 8 * half;
+                    uint32_t words[W];
+                    __half2 pairs[GR];
+                    load_words<W>(tile + r * (D / 2) + kt * (D / 8), words);
+                    load_pairs<GR>(tile + pair_at(D, 0, r, 0), pairs);
+#pragma unroll
+                    for (int w = 0; w < W; ++w) {
+                        const __half2 pair = r < there ? pairs[w / 2] : zero;
+                        const int c = (4 * w + kt) & 7;
+                        ptx::st_shared_v4(base + (uint32_t)((w / 2) * (PN * 128) + r * 128 + ((c ^ (r & 7)) << 4)),
+                                          unpack8(words[w], __low2half2(pair), __high2half2(pair)));
+                    }
+                }
+            }
+            ptx::fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&k_full[buf]);
+            if (!__all_sync(0xffffffffu, ptx::mbar_wait_bounded(&v_empty[buf], ph ^ 1u, abort_flag))) { ok = false; break; }
+            {
+                const uint32_t base = ptx::smem_u32(v_s + buf * Cfg::KV_BYTES) + (uint32_t)(warp * kTileTokens * 128);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int at = i * 4 + (lane >> 3), t = at & 3, c = at >> 2, r = 2 * t + (c & 1) + 8 * (c >> 1);
+                    const int place = lane & 7, chunk = place ^ (2 * t);
+                    uint32_t words[GR];
+                    __half2 pairs[GR];
+                    load_words<GR>(tile + 8 * D + at * (D / 2) + place * (D / 16), words);
+                    load_pairs<GR>(tile + pair_at(D, 1, r, 0), pairs);
+#pragma unroll
+                    for (int w = 0; w < GR; ++w) {
+                        const __half2 pair = r < there ? pairs[w] : zero;
+                        ptx::st_shared_v4(base + (uint32_t)(w * (PN * 128) + r * 128 + ((chunk ^ (r & 7)) << 4)),
+                                          unpack8(words[w], __low2half2(pair), __high2half2(pair)));
+                    }
+                }
+            }
+            ptx::fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&v_full[buf]);
+            issue(j + kRing);
+        }
+        if (!ok) {
+            if (lane == 0) atomicOr(&g_kv4_prefill_status[0], 1u);
+            const uint64_t t0 = ptx::globaltimer_ns();
+            while (ptx::globaltimer_ns() - t0 < 20000ull) {
+            }
+        }
+    } else if (warp == kUnpackWarps) {
+        // ------------------------------ products ----------------------------------
+        if (ptx::elect_one()) {
+            constexpr uint32_t idesc_s = ptx::make_idesc_f16(0, PM, PN, 0);
+            constexpr uint32_t idesc_o = ptx::make_idesc_f16(0, PM, D, 1);
+            bool ok = true;
+            // Score buffer j & 1 of a tile is free without a barrier of its own: block j - 2's P V was issued before, after the
+            // softmax warps had written P, and the tensor core runs this thread's products in order.
+            auto issue_qk = [&](int j) -> bool {
+                const int buf = j & 1;
+                if (!ptx::mbar_wait_bounded(&k_full[buf], (uint32_t)(j >> 1) & 1u, abort_flag)) return false;
+                ptx::tc_fence_after();
+                const uint32_t k_addr = ptx::smem_u32(k_s + buf * Cfg::KV_BYTES);
+                for (int i = 0; i < 2; ++i) {
+                    if (j >= (i ? nblk1 : nblk0)) continue;
+                    if (j == 0 && !ptx::mbar_wait_bounded(&q_full[i], 0, abort_flag)) return false;
+                    if (j == 0) ptx::tc_fence_after();
+                    const uint32_t q_addr = ptx::smem_u32(q_s + i * Cfg::Q_BYTES);
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; ++kk)
+                        ptx::mma_f16_ss(tmem_base + (uint32_t)((2 * i + buf) * PN),
+                                        ptx::make_kmajor_sw128_desc(q_addr + (uint32_t)((kk >> 2) * (PM * 128) + (kk & 3) * 32)),
+                                        ptx::make_kmajor_sw128_desc(k_addr + (uint32_t)((kk >> 2) * (PN * 128) + (kk & 3) * 32)), idesc_s, kk != 0 ? 1u : 0u);
+                    ptx::tc_commit(&s_full[2 * i + buf]);
+                }
+                ptx::tc_commit(&k_empty[buf]);
+                return true;
+            };
+            if (nblk > 0) ok = issue_qk(0);
+            for (int j = 0; j < nblk && ok; ++j) {
+                if (j + 1 < nblk && !issue_qk(j + 1)) { ok = false; break; }
+                const int buf = j & 1;
+                const uint32_t ph = (uint32_t)(j >> 1) & 1u;
+                if (!ptx::mbar_wait_bounded(&v_full[buf], ph, abort_flag)) { ok = false; break; }
+                const uint32_t v_addr = ptx::smem_u32(v_s + buf * Cfg::KV_BYTES);
+                for (int i = 0; i < 2 && ok; ++i) {
+                    const int n = i ? nblk1 : nblk0;
+                    if (j >= n) continue;
+                    if (!ptx::mbar_wait_bounded(&p_full[2 * i + buf], ph, abort_flag)) { ok = false; break; }
+                    ptx::tc_fence_after();
+#pragma unroll
+                    for (int kk = 0; kk < PN / 16; ++kk)  // P: 16 keys = 8 columns of packed pairs per step, over its scores
+                        ptx::mma_f16_ts(tmem_base + 256u + (uint32_t)(i * 128), tmem_base + (uint32_t)((2 * i + buf) * PN + kk * 8),
+                                        ptx::make_mnmajor_sw128_desc(v_addr + (uint32_t)(kk * 16 * 128), PN * 128), idesc_o, (j | kk) != 0 ? 1u : 0u);
+                    ptx::tc_commit(&pv_full[i]);
+                    if (j + 1 == n) ptx::tc_commit(&o_full[i]);
+                }
+                if (ok) ptx::tc_commit(&v_empty[buf]);
+            }
+            if (!ok) {
+                atomicOr(&g_kv4_prefill_status[0], 2u);
+                ptx::tc_commit(drain_bar);
+                const uint64_t t0 = ptx::globaltimer_ns();
+                while (!ptx::mbar_try_wait(drain_bar, 0)) {
+                    if (ptx::globaltimer_ns() - t0 > ptx::kWaitLimitNs) break;
+                }
+            }
+        }
+    } else {
+        // ------------------------------ softmax / output rows ---------------------
+        const int i = (warp - kUnpackWarps - 1) >> 2, quad = warp & 3;
+        const int r_in_tile = quad * 32 + lane;
+        const int n = i ? nblk1 : nblk0;
+        const int lo = u.rt * 2 * PM + i * PM;
+        const int row = lo + r_in_tile;
+        const bool there = u.on && row < rows;
+        const int token = there ? row / p.group : 0;
+        const int head = u.kvh * p.group + (there ? row - token * p.group : 0);
+        const int limit = there ? u.len - u.count + token + 1 : 0x7fffffff;  // keys that the row sees
+        float mul = 0.f;
+        if (n > 0) {
+            // this row of q, a power of two taken out, into the operand tile
+            const T* q = reinterpret_cast<const T*>(p.q) + (int64_t)(u.first + token) * p.q_st + (int64_t)head * p.q_sh;
+            const bool vec = (reinterpret_cast<uintptr_t>(p.q) & 15) == 0 && p.q_st % 8 == 0 && p.q_sh % 8 == 0;
+            uint4 raw[D / 8];
+            float top = 0.f;
+#pragma unroll
+            for (int c = 0; c < D / 8; ++c) {
+                raw[c] = there ? load_q8(q + 8 * c, vec) : make_uint4(0, 0, 0, 0);
+                const T* e = reinterpret_cast<const T*>(&raw[c]);
+#pragma unroll
+                for (int x = 0; x < 8; ++x) top = fmaxf(top, fabsf(Cvt<T>::to_f(e[x])));
+            }
+            int e = (int)(__float_as_uint(top) >> 23) - 127;
+            e = max(-100, min(126, e));
+            float down = __uint_as_float((uint32_t)(127 - e) << 23);
+            if (p.scale == 0.f) down = 0.f;
+            if (p.scale < 0.f) down = -down;
+            mul = fmaxf((p.scale == 0.f ? 1.f : fabsf(p.scale)) * kLog2e * __uint_as_float((uint32_t)(127 + e) << 23), 1e-37f);
+            const uint32_t base = ptx::smem_u32(q_s + i * Cfg::Q_BYTES) + (uint32_t)(r_in_tile * 128);
+#pragma unroll
+            for (int c = 0; c < D / 8; ++c) {
+                const T* e8 = reinterpret_cast<const T*>(&raw[c]);
+                uint32_t w[4];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) w[x] = ptx::pack2<__half>(Cvt<T>::to_f(e8[2 * x]) * down, Cvt<T>::to_f(e8[2 * x + 1]) * down);
+                ptx::st_shared_v4(base + (uint32_t)((c >> 3) * (PM * 128) + (((c & 7) ^ (r_in_tile & 7)) << 4)), make_uint4(w[0], w[1], w[2], w[3]));
+            }
+            ptx::fence_proxy_async();
+            ptx::mbar_arrive(&q_full[i]);
+        }
+        const uint32_t lane_field = (uint32_t)(quad * 32) << 16;
+        const uint32_t o_taddr = tmem_base + lane_field + 256u + (uint32_t)(i * 128);
+        bool ok = true;
+        float m_run = -INFINITY, l_run = 0.f;
+        for (int j = 0; j < n; ++j) {
+            const int buf = j & 1;
+            if (!__all_sync(0xffffffffu, ptx::mbar_wait_bounded(&s_full[2 * i + buf], (uint32_t)(j >> 1) & 1u, abort_flag))) { ok = false; break; }
+            ptx::tc_fence_after();
+            const uint32_t s_taddr = tmem_base + lane_field + (uint32_t)((2 * i + buf) * PN);
+            const int visible = limit - j * PN;  // columns of this block that the row sees
+            int hole = 0;
+#pragma unroll
+            for (int w = 0; w < kUnpackWarps; ++w) hole |= (holes[(j & 3) * kUnpackWarps + w] != 0) << w;
+            if (__all_sync(0xffffffffu, visible <= 0) || hole == 15) {  // probabilities of zero; maximum and sum stay
+                uint32_t zero[32];
+#pragma unroll
+                for (int c = 0; c < 32; ++c) zero[c] = 0u;
+                ptx::tmem_st_32x32(s_taddr, zero);
+                ptx::tmem_st_wait();
+                ptx::tc_fence_before();
+                ptx::mbar_arrive(&p_full[2 * i + buf]);
+                continue;
+            }
+            float sc[PN];
+            {
+                uint32_t r0[32], r1[32];
+                ptx::tmem_ld_32x32(s_taddr, r0);
+                ptx::tmem_ld_32x32(s_taddr + 32u, r1);
+                ptx::tmem_ld_wait();
+#pragma unroll
+                for (int c = 0; c < 32; ++c) {
+                    sc[c] = __uint_as_float(r0[c]);
+                    sc[32 + c] = __uint_as_float(r1[c]);
+                }
+            }
+            if (__any_sync(0xffffffffu, visible < PN) || hole != 0) {
+#pragma unroll
+                for (int c = 0; c < PN; ++c)
+                    if (c >= visible || ((hole >> (c / kTileTokens)) & 1)) sc[c] = -INFINITY;
+            }
+            if (m_run == -INFINITY) {
+                float mxp[8];
+#pragma unroll
+                for (int c = 0; c < 8; ++c) mxp[c] = ptx::fmax3(sc[c], sc[8 + c], sc[16 + c]);
+#pragma unroll
+                for (int at = 24; at < PN; at += 16)
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) mxp[c] = at + 8 < PN ? ptx::fmax3(mxp[c], sc[at + c], sc[at + 8 + c]) : fmaxf(mxp[c], sc[at + c]);
+                m_run = ptx::fmax3(ptx::fmax3(mxp[0], mxp[1], mxp[2]), ptx::fmax3(mxp[3], mxp[4], mxp[5]), fmaxf(mxp[6], mxp[7])) * mul;
+                // (nothing has been added to O yet but zeros, so a first maximum needs no rescaling)
+            }
+            uint32_t pk[32];
+#pragma unroll 1
+            for (int attempt = 0; attempt < 2; ++attempt) {
+                const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
+                float lp[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                float mxp[8];
+#pragma unroll
+                for (int c = 0; c < 8; ++c) mxp[c] = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < PN; c += 2) {
+                    float x0, x1;
+                    ptx::fma2(x0, x1, sc[c], sc[c + 1], mul, mul, neg_m, neg_m);
+                    const int pair = c >> 1;
+                    const float p0 = ptx::ex2_approx(x0), p1 = ptx::ex2_approx(x1);
+                    mxp[pair & 7] = ptx::fmax3(mxp[pair & 7], sc[c], sc[c + 1]);
+                    ptx::add2(lp[2 * (pair & 3)], lp[2 * (pair & 3) + 1], lp[2 * (pair & 3)], lp[2 * (pair & 3) + 1], p0, p1);
+                    pk[pair] = ptx::pack2<__half>(p0, p1);
+                }
+                const float l_blk = ((lp[0] + lp[1]) + (lp[2] + lp[3])) + ((lp[4] + lp[5]) + (lp[6] + lp[7]));
+                if (attempt == 0 && j > 0) {
+                    const float mx = ptx::fmax3(ptx::fmax3(mxp[0], mxp[1], mxp[2]), ptx::fmax3(mxp[3], mxp[4], mxp[5]), fmaxf(mxp[6], mxp[7])) * mul;
+                    const float m_new = fmaxf(m_run, mx);
+                    if (__any_sync(0xffffffffu, m_new > m_run + kLag)) {
+                        const float m_to = m_new == -INFINITY ? 0.f : m_new;
+                        const float alpha = ptx::ex2_approx(m_run - m_to);
+                        if (!__all_sync(0xffffffffu, ptx::mbar_wait_bounded(&pv_full[i], (uint32_t)(j - 1) & 1u, abort_flag))) { ok = false; break; }
+                        ptx::tc_fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < D / 32; ++c) {
+                            uint32_t o[32];
+                            ptx::tmem_ld_32x32(o_taddr + (uint32_t)(c * 32), o);
+                            ptx::tmem_ld_wait();
+#pragma unroll
+                            for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * alpha);
+                            ptx::tmem_st_32x32(o_taddr + (uint32_t)(c * 32), o);
+                        }
+                        l_run *= alpha;
+                        m_run = m_new;
+                        continue;
+                    }
+                }
+                l_run += l_blk;
+                break;
+            }
+            if (!ok) break;
+            ptx::tmem_st_32x32(s_taddr, pk);
+            ptx::tmem_st_wait();
+            ptx::tc_fence_before();
+            ptx::mbar_arrive(&p_full[2 * i + buf]);
+        }
+        if (ok && n > 0) ok = __all_sync(0xffffffffu, ptx::mbar_wait_bounded(&o_full[i], 0, abort_flag)) != 0;
+        if (ok && u.on && lo + quad * 32 < rows) {
+            ptx::tc_fence_after();
+            const float inv_l = l_run > 0.f || l_run != l_run ? 1.0f / l_run : 0.f;
+            // rows leave through a slab of shared memory (this tile's q, which no product reads any more), so that stores are whole lines
+            const uint32_t slab = ptx::smem_u32(q_s + i * Cfg::Q_BYTES) + (uint32_t)(quad * 4096);
+            T* out = reinterpret_cast<T*>(p.out);
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+                uint32_t o[32];
+                if (n > 0) {
+                    ptx::tmem_ld_32x32(o_taddr + (uint32_t)(c * 32), o);
+                    ptx::tmem_ld_wait();
+                } else {
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) o[x] = 0u;
+                }
+#pragma unroll
+                for (int t4 = 0; t4 < 4; ++t4) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) w[x] = ptx::pack2<T>(__uint_as_float(o[t4 * 8 + 2 * x]) * inv_l, __uint_as_float(o[t4 * 8 + 2 * x + 1]) * inv_l);
+                    const int at = (c & 1) * 4 + t4;
+                    ptx::st_shared_v4(slab + (uint32_t)(lane * 128 + ((at ^ (lane & 7)) << 4)), make_uint4(w[0], w[1], w[2], w[3]));
+                }
+                if (c & 1) {
+                    __syncwarp();
+#pragma unroll
+                    for (int it = 0; it < 8; ++it) {
+                        const int r = it * 4 + (lane >> 3), at = lane & 7, row_i = lo + quad * 32 + r;
+                        const uint4 val = ptx::ld_shared_v4(slab + (uint32_t)(r * 128 + ((at ^ (r & 7)) << 4)));
+                        if (row_i < rows) {
+                            const int tk = row_i / p.group, hd = u.kvh * p.group + (row_i - tk * p.group);
+                            *reinterpret_cast<uint4*>(out + ((int64_t)(u.first + tk) * p.heads + hd) * D + (c >> 1) * 64 + at * 8) = val;
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+            ptx::tc_fence_before();
+        }
+        if (!ok && lane == 0) atomicOr(&g_kv4_prefill_status[0], 4u);
+    }
+
+    ptx::tc_fence_before();
+    __syncthreads();
+    if (warp == kUnpackWarps) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc(tmem_base, 512);
+    }
+}
+
+template <typename T, int D>
+int launch_prefill(const AttendParams& p, int beyond, cudaStream_t st) {
+    using Cfg = PreCfg<D>;
+    static std::atomic<uint64_t> reserved;
+    if (!reserve_smem(kv4_prefill_kernel<T, D>, Cfg::SMEM, reserved)) return fail(XG_ERR_LAUNCH, "xg_kv4_attention: cannot reserve shared memory");
+    // at least as many CTAs as there are units; those behind the last one return at once
+    const int64_t grid = (p.tokens * p.group / (2 * PM) + p.batch) * p.cache.heads;
+    if (grid > 0x7fffffffLL) return fail(XG_ERR_TOO_LARGE, "xg_kv4_attention: too many rows");
+    launch_with({.early = false}, kv4_prefill_kernel<T, D>, (unsigned)grid, kPrefillThreads, Cfg::SMEM, st, p, beyond);
+    return check_launch("xg_kv4_attention");
+}
+
+}  // namespace
+
+int attend_prefill(const AttendParams& p, int64_t D, int dtype, int beyond, cudaStream_t st) {
+    if (dtype == XG_BF16) return D == 64 ? launch_prefill<__nv_bfloat16, 64>(p, beyond, st) : launch_prefill<__nv_bfloat16, 128>(p, beyond, st);
+    return D == 64 ? launch_prefill<__half, 64>(p, beyond, st) : launch_prefill<__half, 128>(p, beyond, st);
+}
+
+int read_kv4_prefill_status(unsigned int* host_out, int reset) {
+    unsigned int v[4] = {0, 0, 0, 0};
+    if (cudaMemcpyFromSymbol(v, g_kv4_prefill_status, sizeof(v)) != cudaSuccess) {
+        cudaGetLastError();
+        return fail(XG_ERR_DEVICE, "xg_tc_status: cannot read device status");
+    }
+    *host_out = v[0];
+    if (reset && v[0] != 0) {
+        unsigned int z[4] = {0, 0, 0, 0};
+        cudaMemcpyToSymbol(g_kv4_prefill_status, z, sizeof(z));
+    }
+    return XG_OK;
+}
+}  // namespace xg
