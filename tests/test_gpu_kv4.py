@@ -178,17 +178,21 @@ def _reference(q, cache, table, lens, starts, scale):
         size = torch.einsum("ihd,jhd->hij", qb.abs(), k.abs()).masked_fill(~seen[None], 0.0).amax(-1) * abs(scale)  # of the largest score's terms
         sums = torch.einsum("hij,jhd->ihd", p, v.abs())
         err_k[lo:hi] = sums * size.transpose(0, 1)[..., None]
-        err_v[lo:hi] = sums
+        groups = v.unflatten(-1, (-1, 64))
+        half_range = ((groups.amax(-1) - groups.amin(-1)) / 2)[..., None].expand_as(groups).flatten(-2)
+        err_v[lo:hi] = sums + torch.einsum("hij,jhd->ihd", p, half_range)
     return out, err_k, err_v
 
 
 def _check_attention(got, ref, what, halves=False):
     """Scores: fp32 sums of D products, the terms' size times 2^-20 at most (16 roundings of 2^-24: the tensor core's partial sums).
-    They move a probability by a factor of e^(2 error). The probability itself: two bf16 planes (2^-16) and the exponential
-    (2^-20). `halves`: keys, values and probabilities in fp16 (2^-11 each) instead."""
+    They move a probability by a factor of e^(2 error). The probability times its value's scale goes into the second product as fp16,
+    half a step of 2^-11 off, after the exponential (2^-20) and two fp32 products: that moves the value's distance from the middle of
+    its group's range, at most half the range (8/7.5 of it, as the middle is taken at code 8). What is exact beside it is an fp32 sum.
+    `halves`: keys and values in fp16 too (2^-11 each of the value)."""
     out, err_k, err_v = ref
     assert got.shape == out.shape
-    u_k, u_v = (2.0 ** -11 + 2.0 ** -20, 2 * 2.0 ** -11 + 2.0 ** -19) if halves else (2.0 ** -20, 2.0 ** -15)
+    u_k, u_v = (2.0 ** -11 + 2.0 ** -20, 2 * 2.0 ** -11 + 2.0 ** -19) if halves else (2.0 ** -20, 2.0 ** -11 * 8 / 7.5 + 2.0 ** -19)
     tol = out.abs() * torch.finfo(got.dtype).eps / 2 * (1 + 2.0 ** -6) + 2 * u_k * err_k * (1 + 8 * u_k * err_k) + u_v * err_v + 1e-7
     bad = ~((got.double() - out).abs() <= tol)
     assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, rows {sorted(set(bad.nonzero()[:, 0].tolist()))[:8]}"

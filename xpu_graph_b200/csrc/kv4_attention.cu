@@ -2,6 +2,7 @@
 // ones of sequence b stands at position len_b - n_b + i and sees the keys up to its own. Heads are grouped: query head h reads kv
 // head h / (Hq / Hkv). fp32 scores, softmax and sums.
 #include "kv4_attend.cuh"
+#include <cstdlib>
 
 namespace xg {
 
@@ -16,40 +17,56 @@ using namespace kv4;
 // Few query rows per sequence: the cache streamed once
 // ---------------------------------------------------------------------------------------
 // A unit is a (sequence, kv head, tile of 8 NT columns); its columns are the (new token, head of the group) pairs that read this kv
-// head. The tiles of 16 keys of all units form one line, cut into equal ranges, one per CTA, so that sequences of any mixture of
-// lengths load the chip evenly; what a unit leaves in several CTAs is added by kv4_combine_kernel in range order. A CTA's warps take
-// its tiles in turn, each warp with a ring of bulk copies of its own.
+// head. The 32-key blocks of all units form one line, cut into equal ranges, one per CTA, and those into one per warp, so that
+// sequences of any mixture of lengths load the chip evenly. A warp streams its range through a ring of bulk copies of its own and
+// writes the units that lie wholly in it; what the warps' cuts leave is added in shared memory at the CTA's end, what the CTAs' cuts
+// leave by kv4_combine_kernel, both in range order.
 //
-// Both products run on mma.m16n8k16 with the codes as bf16: a 4-bit code n masked out of its word is the bf16 subnormal n 2^-133 in
-// bits 0-3 and n 2^-129 in bits 4-7 (8 and up carry over into the exponent as they should), which the tensor core multiplies
-// exactly, so unpacking costs one logic operation per two codes and no arithmetic. q and the probabilities carry 2^64 along.
-//   scores (16 keys x 8 columns, per group of 64 channels):  x = scale_k acc + least_k sum(q), the group's sum of q kept per column
-//   output (16 channels x 8 columns):  acc += code (p scale_v), and the sum of p least_v per column and group beside it
-// p scale_v goes in as two bf16 planes (16 bits of significand), q as one for bf16 and two for fp16 (exact).
-// The maximum is kept per column and may lag behind by 2^8; only a larger step rescales the sums.
-// The codes of keys that do not exist are finite whatever they are; their scales are dropped by a select, not a product.
-constexpr int kWarps = 4, kStages = 3;
+// Both products run on mma.m16n8k16 with the codes as fp16: a 4-bit code n masked out of its word is the subnormal n 2^-24 in bits
+// 0-3 and n 2^-20 in bits 4-7, which the tensor core multiplies exactly, so unpacking costs one logic operation per two codes and no
+// arithmetic.
+//   scores (16 keys x 8 columns, per group of 64 channels):  x = scale_k acc + least_k sum(q), the group's sum of q kept per column.
+//     q has a power of two per row taken out, with which bf16 fits fp16 exactly (down to 2^-29 of the row's largest).
+//   output (16 channels x 8 columns):  sum p v = sum w (code - 8) + sum p (least_v + 8 scale_v), w = p scale_v rounded to fp16 (2^-12
+//     relative). The codes go in as they are and 8 sum w comes off at the end, from a product with ones; so what the rounding moves is
+//     in proportion to half the group's range and not to its least value.
+//     w is kept below 2^15 by the power of two that the scales have reached so far; p, up to 2^8, may be 2^29 smaller still.
+// Both that power and the maximum of a column follow their data lagging: only a step beyond them rescales the sums.
+// The codes of keys that do not exist are finite whatever they are; their scales are replaced, not multiplied away.
+//
+// Code that runs once per unit is kept short: fetching it costs more than running it (with a second copy of the loop for masked
+// blocks 64 sequences of 512 to 8192 tokens took 92 us, and of 4096 each 78).
+constexpr int kWarps = 4;
 constexpr int kBlockTiles = 2, kBlockKeys = kBlockTiles * kTileTokens;  // what a stage holds
 constexpr int kMaxBatch = 1024;  // sequences per launch: their prefix sums live in shared memory
 
 // CTAs per SM, by what the fragments and sums take of the register file
 constexpr int split_ctas(int D, int NT) { return D == 256 ? 2 : (NT == 1 ? (D == 64 ? 4 : 3) : (D == 64 ? 3 : 2)); }
 
+// What a warp's range leaves unfinished: the end of a unit that began before it, the beginning of one that goes on behind it (a range
+// inside one unit is an end that does not end).
+struct Cut {
+    int any, head, head_ends, tail;
+    int first, count, kvh, ct, parts;  // of the tail's unit; parts: CTA ranges that it reaches, 1 if it ends in this one
+};
+
 template <int D, int NT>
 struct SplitCfg {
     static constexpr int COLS = 8 * NT;
     static constexpr int TILE = tile_bytes(D);
     static constexpr int STAGE = kBlockTiles * TILE;
-    static constexpr int STAGES = D == 256 ? 2 : kStages;
+    static constexpr int STAGES = 2;
     static constexpr int KT = NT == 1 && D <= 128 ? 2 : 1;  // tiles in work at once: more independent products per warp, more registers
     static constexpr int RING = kWarps * STAGES * STAGE;
     static constexpr int O_STRIDE = D + 4;  // floats
-    static constexpr int O_BYTES = kWarps * COLS * O_STRIDE * 4;
-    static constexpr int ML_BYTES = kWarps * COLS * 2 * 4;
+    static constexpr int SLOT = COLS * O_STRIDE;  // floats of one part in shared memory
+    static constexpr int O_BYTES = kWarps * SLOT * 4;
+    static constexpr int ML_BYTES = 2 * kWarps * COLS * 8;
     static constexpr int BAR_BYTES = kWarps * STAGES * 8;
-    static constexpr int FIXED = RING + O_BYTES + ML_BYTES + BAR_BYTES + kWarps * STAGES * 4 + 64;
+    static constexpr int FIXED = RING + O_BYTES + ML_BYTES + BAR_BYTES + kWarps * (int)sizeof(Cut) + kWarps * STAGES * 4 + 64;
+    static_assert(SLOT * 4 <= STAGES * STAGE, "a warp's ring holds a part");
     static constexpr int part_floats() { return COLS * (D + 2); }
-    static int smem(int batch) { return FIXED + (batch + 1) * 8 + batch * 12; }
+    static int smem(int batch) { return FIXED + (batch + 1) * 4 + batch * 12; }
     static constexpr int CTAS = split_ctas(D, NT);
 };
 
@@ -57,7 +74,7 @@ struct SplitParams {
     AttendParams a;
     float* parts;  // [2 * gridDim.x][COLS][D] sums, then [2 * gridDim.x][COLS] (maximum, sum) pairs, then a PartDesc per CTA
     int split;         // 0: a unit stays in one CTA
-    int64_t min_blocks; // of a range
+    uint32_t min_blocks; // of a range
     int most_cols;       // sequences with more columns are left alone
     int first_rows, last_rows;  // this launch zeroes the rows before the first / behind the last sequence
 };
@@ -68,31 +85,24 @@ struct PartDesc {
     int first, count, kvh, ct, pad[3];
 };
 
-template <typename T>
-struct Planes {
-    static constexpr int N = std::is_same<T, __nv_bfloat16>::value ? 1 : 2;
-};
-
-__device__ __forceinline__ float bf16_lo(uint32_t x) { return __uint_as_float(x << 16); }
-__device__ __forceinline__ float bf16_hi(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
-
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_split_kernel(const SplitParams sp) {
     using Cfg = SplitCfg<D, NT>;
-    constexpr int W = D / 32, GR = D / 64, PL = Planes<T>::N;
+    constexpr int W = D / 32, GR = D / 64;
     const AttendParams& p = sp.a;
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t* ring = smem;
-    float* o_s = reinterpret_cast<float*>(smem + Cfg::RING);
-    float2* ml_s = reinterpret_cast<float2*>(smem + Cfg::RING + Cfg::O_BYTES);
+    float* head_s = reinterpret_cast<float*>(smem + Cfg::RING);  // [warp][COLS][O_STRIDE]; a tail goes where the warp's ring was
+    float2* ml_s = reinterpret_cast<float2*>(smem + Cfg::RING + Cfg::O_BYTES);  // [head, tail][warp][COLS]
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::RING + Cfg::O_BYTES + Cfg::ML_BYTES);
-    int64_t* prefix = reinterpret_cast<int64_t*>(reinterpret_cast<uint8_t*>(bars) + Cfg::BAR_BYTES);  // [batch + 1]
-    int* first_s = reinterpret_cast<int*>(prefix + p.batch + 1);
+    uint32_t* prefix = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(bars) + Cfg::BAR_BYTES);  // [batch + 1]
+    int* first_s = reinterpret_cast<int*>(prefix + p.batch + 1);  // (the host keeps the line below 2^31 blocks)
     int* count_s = first_s + p.batch;
     int* len_s = count_s + p.batch;
     volatile int* hidden_s = len_s + p.batch;  // [kWarps][STAGES], a bit per tile
     volatile int* abort_flag = hidden_s + kWarps * Cfg::STAGES;
-    int64_t* scan_s = reinterpret_cast<int64_t*>(o_s);  // before the first segment only
+    Cut* cut_s = reinterpret_cast<Cut*>(const_cast<int*>(abort_flag + 1));
+    uint32_t* scan_s = reinterpret_cast<uint32_t*>(head_s);  // before the first segment only
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     if (tid == 0) {
@@ -107,27 +117,27 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
     const int kv_heads = p.cache.heads;
     auto col_tiles = [&](int count) { return (count * p.group + Cfg::COLS - 1) / Cfg::COLS; };
     auto blocks_of = [&](int b) { return (len_s[b] + kBlockKeys - 1) / kBlockKeys; };
-    int64_t carry = 0;
+    uint32_t carry = 0;
     for (int base = 0; base < p.batch; base += kWarps * 32) {
         const int b = base + tid;
-        int64_t w = 0;
+        uint32_t w = 0;
         if (b < p.batch) {
             const Sequence s = sequence(p, b);
             first_s[b] = (int)s.first;
             count_s[b] = s.count;
             const int len = s.count * p.group > sp.most_cols ? -1 : (int)s.len;
             len_s[b] = len;
-            w = (int64_t)kv_heads * col_tiles(s.count) * ((max(len, 0) + kBlockKeys - 1) / kBlockKeys);
+            w = len <= 0 ? 0 : (uint32_t)kv_heads * col_tiles(s.count) * ((len + kBlockKeys - 1) / kBlockKeys);
         }
-        int64_t inc = w;
+        uint32_t inc = w;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int64_t v = __shfl_up_sync(0xffffffffu, inc, o);
+            const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
             if (lane >= o) inc += v;
         }
         if (lane == 31) scan_s[warp] = inc;
         __syncthreads();
-        int64_t before = carry, all = carry;
+        uint32_t before = carry, all = carry;
 #pragma unroll
         for (int i = 0; i < kWarps; ++i) {
             if (i < warp) before += scan_s[i];
@@ -139,7 +149,7 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
     }
     if (tid == 0) prefix[p.batch] = carry;
     __syncthreads();
-    const int64_t total = carry;
+    const uint32_t total = carry;
 
     // rows that no key reaches because there is no sequence, or nothing in its cache
     {
@@ -155,10 +165,12 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
             if (len_s[b] == 0) zero(first_s[b], (int64_t)first_s[b] + count_s[b], 0, 1);
     }
 
-    int64_t ranges = (total + sp.min_blocks - 1) / sp.min_blocks;
+    uint32_t ranges = (total + sp.min_blocks - 1) / sp.min_blocks;
     if (ranges > gridDim.x) ranges = gridDim.x;
-    int64_t start = 0, end = 0;
-    auto sequence_at = [&](int64_t x) {  // the b with prefix[b] <= x < prefix[b + 1]
+    const uint32_t share = ranges ? total / ranges : 0, over = total - share * ranges;
+    auto range_at = [&](uint32_t i) { return share * i + (i < over ? i : over); };  // where range i starts
+    uint32_t start = 0, end = 0;
+    auto sequence_at = [&](uint32_t x) {  // the b with prefix[b] <= x < prefix[b + 1]
         int lo = 0, hi = p.batch - 1;
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
@@ -167,14 +179,14 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
         }
         return lo;
     };
-    if ((int64_t)blockIdx.x < ranges) {
-        start = total * blockIdx.x / ranges;
-        end = total * (blockIdx.x + 1) / ranges;
+    if (blockIdx.x < ranges) {
+        start = range_at(blockIdx.x);
+        end = range_at(blockIdx.x + 1);
         if (!sp.split) {
-            auto up = [&](int64_t x) {
+            auto up = [&](uint32_t x) {
                 if (x >= total) return total;
                 const int b = sequence_at(x);
-                const int64_t n = blocks_of(b), off = x - prefix[b];
+                const uint32_t n = blocks_of(b), off = x - prefix[b];
                 return prefix[b] + (off + n - 1) / n * n;
             };
             start = up(start);
@@ -185,22 +197,24 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
     if (sp.split && tid == 0) desc->parts = 0;
     if (start >= end) return;
 
-    // ---- this warp's tiles: start + warp + 4 i
-    const int mine = (int)((end - start - warp + kWarps - 1) / kWarps);
+    // ---- this warp's blocks
+    const uint32_t quarter = (end - start) / kWarps, left = (end - start) % kWarps;
+    const uint32_t my_start = start + quarter * warp + min((uint32_t)warp, left), my_end = my_start + quarter + (warp < left ? 1 : 0);
+    const int mine = (int)(my_end - my_start);
     uint8_t* my_ring = ring + warp * (Cfg::STAGES * Cfg::STAGE);
     uint64_t* my_bars = bars + warp * Cfg::STAGES;
     volatile int* my_hidden = hidden_s + warp * Cfg::STAGES;
     // where this lane's block of the current batch of 32 lies, tile by tile; 0 where there is nothing to read
     int64_t addr[kBlockTiles] = {};
     auto look_up = [&](int i) {
-        const int64_t x = start + warp + (int64_t)kWarps * (i + lane);
+        const uint32_t x = my_start + i + lane;
 #pragma unroll
         for (int k = 0; k < kBlockTiles; ++k) addr[k] = 0;
-        if (x >= end) return;
+        if (x >= my_end) return;
         const int b = sequence_at(x);
-        const int64_t n = blocks_of(b), off = x - prefix[b];
-        const int64_t unit = off / n;
-        const int kvh = (int)(unit / col_tiles(count_s[b]));
+        const uint32_t n = blocks_of(b), off = x - prefix[b];
+        const uint32_t unit = off / n;
+        const int kvh = (int)(unit / (uint32_t)col_tiles(count_s[b]));
 #pragma unroll
         for (int k = 0; k < kBlockTiles; ++k) {
             const int tile = (int)(off - unit * n) * kBlockTiles + k;
@@ -234,27 +248,27 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
     };
     for (int i = 0; i < Cfg::STAGES; ++i) issue(i, i);
 
-    // Scores stay in the units of the products (2^-69 / scale) up to the exponent; a negative scale goes into q, a zero one makes q zero.
+    // a negative scale goes into q, a zero one makes q zero
     const float q_mul = p.scale > 0.f ? 1.f : (p.scale < 0.f ? -1.f : (p.scale == 0.f ? 0.f : p.scale));
-    const float to_log2 = (p.scale != 0.f ? fabsf(p.scale) : 1.f) * kLog2e * 0x1p69f;
-    const float step = 8.f / to_log2;
+    const float scale_log2 = (p.scale != 0.f ? fabsf(p.scale) : 1.f) * kLog2e;
     int done = 0, stage = 0;  // tiles of this warp consumed, and the stage of the next one
     uint32_t phase = 0;
     bool ok = true;
-    int b = sequence_at(start);
-    for (int64_t pos = start; pos < end && ok;) {
+    Cut cut = {mine > 0};
+    int b = mine > 0 ? sequence_at(my_start) : 0;
+    for (uint32_t pos = my_start; pos < my_end && ok;) {
         while (prefix[b + 1] <= pos) ++b;
         const int n_blocks = blocks_of(b), count = count_s[b], len = len_s[b];
-        const int64_t off = pos - prefix[b];
-        const int64_t unit = off / n_blocks;
+        const uint32_t off = pos - prefix[b];
+        const uint32_t unit = off / (uint32_t)n_blocks;
         const int t0 = (int)(off - unit * n_blocks);  // blocks, as n_blocks and seg
         const int cts = col_tiles(count);
-        const int kvh = (int)(unit / cts), ct = (int)(unit - (int64_t)kvh * cts);
-        const int seg = (int)(n_blocks - t0 < end - pos ? n_blocks - t0 : end - pos);
+        const int kvh = (int)(unit / (uint32_t)cts), ct = (int)(unit - (uint32_t)kvh * cts);
+        const int seg = min(n_blocks - t0, (int)(my_end - pos));
 
         // ---- q as fragments; column n = 8 nt + g is the pair (new token col / group, head col % group)
-        uint32_t qf[NT][PL][W][4];  // [.][.][w][2 h + i]: fragment register i of k-step 2 w + h
-        float qsum[NT][GR][2];
+        uint32_t qf[NT][W][4];  // [.][w][2 h + i]: fragment register i of k-step 2 w + h
+        float qsum[NT][GR][2], to_log2[NT][2];
         int limit[NT][2];
         int least_limit = 0x7fffffff;
         {
@@ -267,8 +281,18 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
                 const int token = col / p.group, head = kvh * p.group + (col - token * p.group);
                 const T* row = q + (int64_t)(first_s[b] + token) * p.q_st + (int64_t)head * p.q_sh + 8 * t;
                 uint4 raw[W];
+                float top = 0.f;
 #pragma unroll
-                for (int w = 0; w < W; ++w) raw[w] = on ? load_q8(row + 32 * w, vec) : make_uint4(0, 0, 0, 0);
+                for (int w = 0; w < W; ++w) {
+                    raw[w] = on ? load_q8(row + 32 * w, vec) : make_uint4(0, 0, 0, 0);
+                    const T* e = reinterpret_cast<const T*>(&raw[w]);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(Cvt<T>::to_f(e[i])));
+                }
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const int e2 = max(-100, min(100, (int)(__float_as_uint(top) >> 23) - 127));  // the row is carried below 2^15
+                const float up = q_mul * __uint_as_float((uint32_t)(127 + 14 - e2) << 23);
 #pragma unroll
                 for (int gr = 0; gr < GR; ++gr) {
                     float sum = 0.f;
@@ -278,44 +302,44 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
                         const T* e = reinterpret_cast<const T*>(&raw[w]);
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
-                            x[i] = Cvt<T>::to_f(e[i]) * q_mul;
+                            x[i] = Cvt<T>::to_f(e[i]) * up;
                             sum += x[i];
-                            // odd codes are 16 times as heavy as they should be
-                            x[i] *= (i & 1) ? 0x1p60f : 0x1p64f;
+                            if (i & 1) x[i] *= 0x1p-4f;  // odd codes are 16 times as heavy as they should be
                         }
 #pragma unroll
                         for (int h = 0; h < 2; ++h)
 #pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                const float lo = x[2 * h + i], hi = x[2 * h + i + 4];
-                                const uint32_t top = ptx::pack2<__nv_bfloat16>(lo, hi);
-                                qf[nt][0][w][2 * h + i] = top;
-                                if (PL == 2) qf[nt][PL - 1][w][2 * h + i] = ptx::pack2<__nv_bfloat16>(lo - bf16_lo(top), hi - bf16_hi(top));
-                            }
+                            for (int i = 0; i < 2; ++i) qf[nt][w][2 * h + i] = ptx::pack2<__half>(x[2 * h + i], x[2 * h + i + 4]);
                     }
                     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) qsum[nt][gr][c] = 0x1p-69f * __shfl_sync(0xffffffffu, sum, (2 * t + c) * 4);
+                    for (int c = 0; c < 2; ++c) qsum[nt][gr][c] = 0x1p-24f * __shfl_sync(0xffffffffu, sum, (2 * t + c) * 4);
                 }
+                const float back = fmaxf(scale_log2 * __uint_as_float((uint32_t)(127 + 10 + e2) << 23), 1e-37f);
                 const int lim = on ? len - count + token + 1 : 0x7fffffff;  // keys that the column sees
                 least_limit = min(least_limit, lim);
 #pragma unroll
-                for (int c = 0; c < 2; ++c) limit[nt][c] = __shfl_sync(0xffffffffu, lim, (2 * t + c) * 4);
+                for (int c = 0; c < 2; ++c) {
+                    to_log2[nt][c] = __shfl_sync(0xffffffffu, back, (2 * t + c) * 4);
+                    limit[nt][c] = __shfl_sync(0xffffffffu, lim, (2 * t + c) * 4);
+                }
             }
             least_limit = __reduce_min_sync(0xffffffffu, least_limit);
         }
-        // m: largest score; bar: what a score has to exceed for m to follow; use: the exponent's offset. Probabilities carry 2^64.
-        float m[NT][2], bar[NT][2], use[NT][2], l[NT][2], low[NT][GR][2], acc[NT][2 * W][4];
+        // m: largest score; bar: what a score has to exceed for m to follow; use: the exponent's offset
+        float m[NT][2], bar[NT][2], use[NT][2], l[NT][2], low[NT][GR][2], eight[NT][GR][4], acc[NT][2 * W][4];
+        float v_exp = -40.f;               // of the values' scales so far: none exceeds 2^v_exp
+        __half v_bar = __ushort_as_half(0);  // 2^v_exp
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 m[nt][c] = bar[nt][c] = -INFINITY;
-                use[nt][c] = 64.f;
+                use[nt][c] = 7.f - v_exp;
                 l[nt][c] = 0.f;
 #pragma unroll
-                for (int gr = 0; gr < GR; ++gr) low[nt][gr][c] = 0.f;
+                for (int gr = 0; gr < GR; ++gr) low[nt][gr][c] = eight[nt][gr][c] = eight[nt][gr][2 + c] = 0.f;
             }
 #pragma unroll
             for (int i = 0; i < 2 * W; ++i)
@@ -323,12 +347,18 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
                 for (int e = 0; e < 4; ++e) acc[nt][i][e] = 0.f;
         }
 
-        // KT tiles; MASKED: some key of theirs is not there for some column
-        auto work = [&](const uint8_t* tile, const int key0, const int hidden, auto masked) {
-            constexpr bool MASKED = decltype(masked)::value;
+        const int seg_at = (int)(pos - my_start);  // of the range
+        for (; done < seg_at + seg; ++done) {
+            if (!__all_sync(0xffffffffu, wait_stage(&my_bars[stage], phase, abort_flag))) { ok = false; break; }
+            const int hidden_tiles = my_hidden[stage];
+#pragma unroll 1
+            for (int k0 = 0; k0 < kBlockTiles; k0 += Cfg::KT) {
             constexpr int KT = Cfg::KT;
+            const int key0 = (t0 + done - seg_at) * kBlockKeys + k0 * kTileTokens, hidden = hidden_tiles >> k0;
+            const uint8_t* tile = my_ring + stage * Cfg::STAGE + k0 * Cfg::TILE;
+            const bool masked = key0 + KT * kTileTokens > least_limit || hidden != 0;  // some key is not there for some column; uniform over the warp
             // ---- scores
-            __half2 kp[KT][2][GR];  // this lane's two keys' pairs
+            __half2 kp[KT][2][GR], vp[KT][2][GR];  // this lane's two keys' pairs
             uint32_t ka[KT][W], kb[KT][W];
 #pragma unroll
             for (int k = 0; k < KT; ++k) {
@@ -336,7 +366,10 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
                 load_words<W>(kr, ka[k]);
                 load_words<W>(kr + 4 * D, kb[k]);
 #pragma unroll
-                for (int r = 0; r < 2; ++r) load_pairs<GR>(tile + k * Cfg::TILE + pair_at(D, 0, g + 8 * r, 0), kp[k][r]);
+                for (int r = 0; r < 2; ++r) {
+                    load_pairs<GR>(tile + k * Cfg::TILE + pair_at(D, 0, g + 8 * r, 0), kp[k][r]);
+                    load_pairs<GR>(tile + k * Cfg::TILE + pair_at(D, 1, g + 8 * r, 0), vp[k][r]);
+                }
             }
             float sc[KT][NT][4];
 #pragma unroll
@@ -351,12 +384,10 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
                             const uint32_t ua = ka[k][w] >> (8 * h), ub = kb[k][w] >> (8 * h);
                             const uint32_t a0 = ua & 0x000f000fu, a1 = ub & 0x000f000fu, a2 = ua & 0x00f000f0u, a3 = ub & 0x00f000f0u;
 #pragma unroll
-                            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                                for (int pl = 0; pl < PL; ++pl) {
-                                    if (w == 2 * gr && h == 0 && pl == 0) ptx::mma_bf16_16816_first(d[k][nt], a0, a1, a2, a3, qf[nt][pl][w][0], qf[nt][pl][w][1]);
-                                    else ptx::mma_bf16_16816(d[k][nt], a0, a1, a2, a3, qf[nt][pl][w][2 * h], qf[nt][pl][w][2 * h + 1]);
-                                }
+                            for (int nt = 0; nt < NT; ++nt) {
+                                if (w == 2 * gr && h == 0) ptx::mma_f16_16816_first(d[k][nt], a0, a1, a2, a3, qf[nt][w][0], qf[nt][w][1]);
+                                else ptx::mma_f16_16816(d[k][nt], a0, a1, a2, a3, qf[nt][w][2 * h], qf[nt][w][2 * h + 1]);
+                            }
                         }
 #pragma unroll
                 for (int k = 0; k < KT; ++k) {
@@ -374,17 +405,25 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
                         }
                 }
             }
-            auto visible = [&](int k, int nt, int e) {
-                return ((hidden >> k) & 1) == 0 && key0 + k * kTileTokens + g + (e & 2) * 4 < limit[nt][e & 1];
-            };
-            if (MASKED) {
+            uint32_t seen = 0xffffffffu;  // a bit per (tile, column tile, element)
+            if (masked) {
 #pragma unroll
-                for (int k = 0; k < KT; ++k)
+                for (int k = 0; k < KT; ++k) {
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
+                    for (int r = 0; r < 2; ++r) {
+                        const bool there = ((hidden >> k) & 1) == 0 && key0 + k * kTileTokens + g + 8 * r < len;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (!visible(k, nt, e)) sc[k][nt][e] = -INFINITY;
+                        for (int gr = 0; gr < GR; ++gr) vp[k][r][gr] = there ? vp[k][r][gr] : __half2half2(__ushort_as_half(0));
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int c = 0; c < 2; ++c)
+                                if (!(there && key0 + k * kTileTokens + g + 8 * r < limit[nt][c])) {
+                                    seen &= ~(1u << ((k * NT + nt) * 4 + 2 * r + c));
+                                    sc[k][nt][2 * r + c] = -INFINITY;
+                                }
+                    }
+                }
             }
             // ---- softmax
             float mx[NT][2];
@@ -397,7 +436,24 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
                     if (KT == 2) mx[nt][c] = ptx::fmax3(mx[nt][c], sc[KT - 1][nt][c], sc[KT - 1][nt][2 + c]);
                     grow = grow || mx[nt][c] > bar[nt][c];
                 }
+            __half2 v_top = __half2half2(__ushort_as_half(0));  // largest scale of the values (low half)
+#pragma unroll
+            for (int k = 0; k < KT; ++k)
+#pragma unroll
+                for (int r = 0; r < 2; ++r)
+#pragma unroll
+                    for (int gr = 0; gr < GR; ++gr) v_top = __hmax2(v_top, vp[k][r][gr]);
+            grow = grow || __hgt(__low2half(v_top), v_bar);
             if (__any_sync(0xffffffffu, grow)) {
+                float v_new = v_exp;
+                {
+                    float top = __low2float(v_top);
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    // the power of two above it; fp16's largest stands for 2^16
+                    if (top > 0.f) v_new = fmaxf(v_exp, (float)((int)(__float_as_uint(top) >> 23) - 126));
+                    v_bar = __float2half_rz(v_new < -24.f ? 0.f : __uint_as_float((uint32_t)(127 + (int)v_new) << 23));
+                }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -406,20 +462,25 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                        const float to = fmaxf(m[nt][c], top);
-                        const float alpha = to == -INFINITY ? 1.f : ptx::ex2_approx((m[nt][c] - to) * to_log2);
+                        const float to = top > bar[nt][c] ? top : m[nt][c];
+                        const float use_new = (to == -INFINITY ? 7.f : fmaf(-to, to_log2[nt][c], 7.f)) - v_new;
+                        const float alpha = m[nt][c] == -INFINITY ? 1.f : ptx::ex2_approx(use_new - use[nt][c]);
                         m[nt][c] = to;
-                        bar[nt][c] = to + step;
-                        use[nt][c] = to == -INFINITY ? 64.f : fmaf(-to, to_log2, 64.f);
+                        bar[nt][c] = to == -INFINITY ? to : to + 8.f / to_log2[nt][c];
+                        use[nt][c] = use_new;
                         l[nt][c] *= alpha;
 #pragma unroll
-                        for (int gr = 0; gr < GR; ++gr) low[nt][gr][c] *= alpha;
+                        for (int gr = 0; gr < GR; ++gr) {
+                            low[nt][gr][c] *= alpha;
+                            eight[nt][gr][c] *= alpha;
+                        }
 #pragma unroll
                         for (int i = 0; i < 2 * W; ++i) {
                             acc[nt][i][c] *= alpha;
                             acc[nt][i][2 + c] *= alpha;
                         }
                     }
+                v_exp = v_new;
             }
             float pr[KT][NT][4];
 #pragma unroll
@@ -428,53 +489,41 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int r = 0; r < 4; r += 2) {
-                        float x0, x1;
-                        ptx::fma2(x0, x1, sc[k][nt][r], sc[k][nt][r + 1], to_log2, to_log2, use[nt][0], use[nt][1]);
-                        pr[k][nt][r] = ptx::ex2_approx(x0);
-                        pr[k][nt][r + 1] = ptx::ex2_approx(x1);
-                        ptx::add2(l[nt][0], l[nt][1], l[nt][0], l[nt][1], pr[k][nt][r], pr[k][nt][r + 1]);
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            pr[k][nt][r + c] = ptx::ex2_approx(fmaf(sc[k][nt][r + c], to_log2[nt][c], use[nt][c]));
+                            l[nt][c] += pr[k][nt][r + c];
+                        }
                     }
             // ---- output
 #pragma unroll
             for (int k = 0; k < KT; ++k) {
                 uint32_t v[4][GR];
-                __half2 vp[2][GR];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) load_words<GR>(tile + k * Cfg::TILE + 8 * D + (4 * c + t) * (D / 2) + (g ^ (2 * t)) * (D / 16), v[c]);
 #pragma unroll
-                for (int r = 0; r < 2; ++r) load_pairs<GR>(tile + k * Cfg::TILE + pair_at(D, 1, g + 8 * r, 0), vp[r]);
-#pragma unroll
                 for (int gr = 0; gr < GR; ++gr) {
-                    const float2 pa = __half22float2(vp[0][gr]), pb = __half22float2(vp[1][gr]);
-                    uint32_t f[NT][2][2];  // [.][plane][keys 0-7, 8-15]
+                    const float2 pa = __half22float2(vp[k][0][gr]), pb = __half22float2(vp[k][1][gr]);
+                    const float mid_a = fmaf(8.f, pa.x, pa.y), mid_b = fmaf(8.f, pb.x, pb.y);
+                    uint32_t f[NT][2];  // [.][keys 0-7, 8-15]
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        float w[4];
-                        if (MASKED) {  // (a hidden key's scale may be anything)
+                        float w[4], y[4];
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const bool on = visible(k, nt, e);
-                                w[e] = on ? pr[k][nt][e] * ((e & 2) ? pb.x : pa.x) : 0.f;
-                                low[nt][gr][e & 1] += on ? pr[k][nt][e] * ((e & 2) ? pb.y : pa.y) : 0.f;
-                            }
-                        } else {
+                        for (int x = 0; x < 4; ++x) {
+                            w[x] = pr[k][nt][x] * ((x & 2) ? pb.x : pa.x);
+                            y[x] = pr[k][nt][x] * ((x & 2) ? mid_b : mid_a);
+                        }
+                        if (masked) {  // (a key may be there for one column and hidden, with NaN in its values, for another)
 #pragma unroll
-                            for (int r = 0; r < 4; r += 2) {
-                                const float least = r ? pb.y : pa.y, scale = r ? pb.x : pa.x;
-#pragma unroll
-                                for (int c = 0; c < 2; ++c) {
-                                    w[r + c] = pr[k][nt][r + c] * scale;
-                                    low[nt][gr][c] = fmaf(pr[k][nt][r + c], least, low[nt][gr][c]);
-                                }
-                            }
+                            for (int x = 0; x < 4; ++x)
+                                if (!((seen >> ((k * NT + nt) * 4 + x)) & 1u)) w[x] = y[x] = 0.f;
                         }
 #pragma unroll
-                        for (int r = 0; r < 2; ++r) {
-                            const uint32_t top = ptx::pack2<__nv_bfloat16>(w[2 * r], w[2 * r + 1]);
-                            const uint32_t rest = ptx::pack2<__nv_bfloat16>(w[2 * r] - bf16_lo(top), w[2 * r + 1] - bf16_hi(top));
-                            f[nt][0][r] = ptx::transpose_8x8(top);
-                            f[nt][1][r] = ptx::transpose_8x8(rest);
-                        }
+                        for (int c = 0; c < 2; ++c) low[nt][gr][c] += y[c] + y[2 + c];
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) f[nt][r] = ptx::transpose_8x8(ptx::pack2<__half>(w[2 * r], w[2 * r + 1]));
+                        ptx::mma_f16_16816(eight[nt][gr], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, f[nt][0], f[nt][1]);
                     }
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
@@ -486,28 +535,14 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
                             const uint32_t a0 = x01 & 0x000f000fu, a1 = x01 & 0x00f000f0u, a2 = x23 & 0x000f000fu, a3 = x23 & 0x00f000f0u;
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                                for (int pl = 0; pl < 2; ++pl)
-                                    ptx::mma_bf16_16816(acc[nt][4 * gr + 2 * half + h], a0, a1, a2, a3, f[nt][pl][0], f[nt][pl][1]);
+                                ptx::mma_f16_16816(acc[nt][4 * gr + 2 * half + h], a0, a1, a2, a3, f[nt][0], f[nt][1]);
                         }
                     }
                 }
             }
-        };
-        const int seg_at = (int)(pos - start);  // of the range
-        for (int at = warp + kWarps * done - seg_at; at < seg; at += kWarps) {
-            if (!__all_sync(0xffffffffu, wait_stage(&my_bars[stage], phase, abort_flag))) { ok = false; break; }
-            const int hidden = my_hidden[stage];
-#pragma unroll 1
-            for (int k0 = 0; k0 < kBlockTiles; k0 += Cfg::KT) {
-                const int key0 = (t0 + at) * kBlockKeys + k0 * kTileTokens;
-                const uint8_t* tile = my_ring + stage * Cfg::STAGE + k0 * Cfg::TILE;
-                if (key0 + Cfg::KT * kTileTokens > least_limit || (hidden >> k0) != 0) work(tile, key0, hidden >> k0, std::true_type{});  // uniform over the warp
-                else work(tile, key0, 0, std::false_type{});
             }
             __syncwarp();  // every lane has read the stage
             issue(done + Cfg::STAGES, stage);
-            ++done;
             if (++stage == Cfg::STAGES) {
                 stage = 0;
                 phase ^= 1u;
@@ -515,7 +550,10 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
         }
         if (!ok) break;
 
-        // ---- the warps' sums of this segment together
+        // ---- the unit's columns, or this range's part of them
+        const bool whole = seg == n_blocks;
+        const int at_end = t0 == 0 ? 1 : 0;  // a part: tail or head
+        float* part = at_end ? reinterpret_cast<float*>(my_ring) : head_s + warp * Cfg::SLOT;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -526,41 +564,80 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
 #pragma unroll
                     for (int gr = 0; gr < GR; ++gr) low[nt][gr][c] += __shfl_xor_sync(0xffffffffu, low[nt][gr][c], o);
                 }
-                if (g == 0) ml_s[warp * Cfg::COLS + nt * 8 + 2 * t + c] = make_float2(m[nt][c] * to_log2, l[nt][c]);
+                const int col = nt * 8 + 2 * t + c;
+                if (!whole && g == 0) ml_s[(at_end * kWarps + warp) * Cfg::COLS + col] = make_float2(m[nt][c] == -INFINITY ? m[nt][c] : -use[nt][c], l[nt][c]);
+                const int pair = ct * Cfg::COLS + col, token = pair / p.group, head = kvh * p.group + (pair - token * p.group);
+                T* out = reinterpret_cast<T*>(p.out) + ((int64_t)(first_s[b] + token) * p.heads + head) * D + 8 * g;
 #pragma unroll
-                for (int i = 0; i < 2 * W; ++i) {  // block i: channels 64 (i / 4) + 8 g + 2 (i % 4) + {0, 1}
-                    const float base = low[nt][i / 4][c];
-                    const float2 y = make_float2(fmaf(acc[nt][i][c] * 0x1p69f, 0x1p64f, base), fmaf(acc[nt][i][2 + c] * 0x1p65f, 0x1p64f, base));
-                    *reinterpret_cast<float2*>(o_s + (warp * Cfg::COLS + nt * 8 + 2 * t + c) * Cfg::O_STRIDE + 64 * (i / 4) + 8 * g + 2 * (i & 3)) = y;
+                for (int gr = 0; gr < GR; ++gr) {  // channels 64 gr + 8 g + {0 .. 7}: two of each of four blocks
+                    float y[8];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        y[2 * i] = fmaf(acc[nt][4 * gr + i][c] - eight[nt][gr][c], 0x1p24f, low[nt][gr][c]);
+                        y[2 * i + 1] = fmaf(acc[nt][4 * gr + i][2 + c] - 16.f * eight[nt][gr][c], 0x1p20f, low[nt][gr][c]);
+                    }
+                    if (whole) {
+                        if (pair < count * p.group) store_row8<T>(out + 64 * gr, y, l[nt][c]);
+                    } else {
+                        float4* dst = reinterpret_cast<float4*>(part + col * Cfg::O_STRIDE + 64 * gr + 8 * g);
+                        dst[0] = make_float4(y[0], y[1], y[2], y[3]);
+                        dst[1] = make_float4(y[4], y[5], y[6], y[7]);
+                    }
                 }
             }
-        __syncthreads();
-        if (*abort_flag) { ok = false; break; }
-        const bool whole = seg == n_blocks;
-        const int64_t slot = 2 * (int64_t)blockIdx.x + (t0 == 0 ? 1 : 0);
-        const int cols = min(Cfg::COLS, count * p.group - ct * Cfg::COLS);
+        if (!whole && at_end) {
+            cut.tail = 1;
+            cut.first = first_s[b]; cut.count = count; cut.kvh = kvh; cut.ct = ct;
+            cut.parts = 1;
+            while (sp.split && range_at(blockIdx.x + cut.parts) < pos + n_blocks) ++cut.parts;
+        } else if (!whole) {
+            cut.head = 1;
+            cut.head_ends = t0 + seg == n_blocks;
+        }
+        pos += seg;
+    }
+    if (lane == 0) cut_s[warp] = cut;
+    __syncthreads();
+    if (*abort_flag) ok = false;
+
+    // ---- what the warps' cuts left: heads that belong to an earlier CTA's unit, then every tail with the heads behind it
+    for (int a = -1; a < kWarps && ok; ++a) {
+        if (a >= 0 && !cut_s[a].tail) continue;
+        uint32_t heads = 0;
+        bool ended = false;
+        for (int w = a + 1; w < kWarps && !ended; ++w) {
+            if (!cut_s[w].any) continue;
+            if (!cut_s[w].head) break;
+            heads |= 1u << w;
+            ended = cut_s[w].head_ends != 0;
+        }
+        if (a < 0 && heads == 0) continue;
+        const Cut u = cut_s[a < 0 ? 0 : a];
+        const bool here = a >= 0 && ended;  // all of the unit
+        const int64_t slot = 2 * (int64_t)blockIdx.x + (a >= 0 ? 1 : 0);
+        const int cols = a >= 0 ? min(Cfg::COLS, u.count * p.group - u.ct * Cfg::COLS) : Cfg::COLS;
         for (int i = tid; i < cols * (D / 8); i += kWarps * 32) {
             const int col = i / (D / 8), ch = (i - col * (D / 8)) * 8;
-            float mx = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, ml_s[w * Cfg::COLS + col].x);
-            const float use = mx == -INFINITY ? 0.f : mx;
+            float mx = a >= 0 ? ml_s[(kWarps + a) * Cfg::COLS + col].x : -INFINITY;
+            for (int w = 0; w < kWarps; ++w)
+                if ((heads >> w) & 1) mx = fmaxf(mx, ml_s[w * Cfg::COLS + col].x);
+            const float to = mx == -INFINITY ? 0.f : mx;
             float sum = 0.f, o[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) o[e] = 0.f;
+#pragma unroll 1
+            for (int w = a < 0 ? 0 : a; w < kWarps; ++w) {
+                if (w != a && !((heads >> w) & 1)) continue;
+                const float2 ml = ml_s[(w == a ? kWarps + w : w) * Cfg::COLS + col];
+                const float f = ptx::ex2_approx(ml.x - to);
+                sum = fmaf(ml.y, f, sum);
+                const float* src = (w == a ? reinterpret_cast<const float*>(ring + w * (Cfg::STAGES * Cfg::STAGE)) : head_s + w * Cfg::SLOT) + col * Cfg::O_STRIDE + ch;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float2 part = ml_s[w * Cfg::COLS + col];
-                const float f = ptx::ex2_approx(part.x - use);
-                sum = fmaf(part.y, f, sum);
-                const float4* src = reinterpret_cast<const float4*>(o_s + (w * Cfg::COLS + col) * Cfg::O_STRIDE + ch);
-                const float4 a = src[0], c = src[1];
-                o[0] = fmaf(a.x, f, o[0]); o[1] = fmaf(a.y, f, o[1]); o[2] = fmaf(a.z, f, o[2]); o[3] = fmaf(a.w, f, o[3]);
-                o[4] = fmaf(c.x, f, o[4]); o[5] = fmaf(c.y, f, o[5]); o[6] = fmaf(c.z, f, o[6]); o[7] = fmaf(c.w, f, o[7]);
+                for (int e = 0; e < 8; ++e) o[e] = fmaf(src[e], f, o[e]);
             }
-            if (whole) {
-                const int at = ct * Cfg::COLS + col, token = at / p.group, head = kvh * p.group + (at - token * p.group);
-                store_row8<T>(reinterpret_cast<T*>(p.out) + ((int64_t)(first_s[b] + token) * p.heads + head) * D + ch, o, sum);
+            if (here) {
+                const int pair = u.ct * Cfg::COLS + col, token = pair / p.group, head = u.kvh * p.group + (pair - token * p.group);
+                store_row8<T>(reinterpret_cast<T*>(p.out) + ((int64_t)(u.first + token) * p.heads + head) * D + ch, o, sum);
             } else {
                 float4* dst = reinterpret_cast<float4*>(sp.parts + (slot * Cfg::COLS + col) * D + ch);
                 dst[0] = make_float4(o[0], o[1], o[2], o[3]);
@@ -568,14 +645,7 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
                 if (ch == 0) reinterpret_cast<float2*>(sp.parts + (int64_t)2 * gridDim.x * Cfg::COLS * D)[slot * Cfg::COLS + col] = make_float2(mx, sum);
             }
         }
-        if (!whole && t0 == 0 && tid == 0) {  // the unit goes on in the next ranges
-            const int64_t unit_end = pos + n_blocks;
-            int parts = 1;
-            while (total * ((int64_t)blockIdx.x + parts) / ranges < unit_end) ++parts;
-            *desc = {parts, first_s[b], count, kvh, ct, {0, 0, 0}};
-        }
-        __syncthreads();
-        pos += seg;
+        if (a >= 0 && !here && tid == 0) *desc = {u.parts, u.first, u.count, u.kvh, u.ct, {0, 0, 0}};  // the unit goes on in the next ranges
     }
     if (!ok) {  // a copy did not arrive in time: what is in flight gets a bounded time to land before shared memory is given up
         if (tid == 0) atomicOr(&g_kv4_status[0], 1u);
@@ -585,78 +655,87 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
     }
 }
 
-// The parts of the unit that starts in range blockIdx.x and goes on in others: out = sum 2^(m_i - m) O_i / sum 2^(m_i - m) l_i, a CTA
-// per column, its warps take the parts in turn.
+// The parts of the unit that starts in range blockIdx.x and goes on in others: out = sum 2^(m_i - m) O_i / sum 2^(m_i - m) l_i. A CTA per
+// range (most have nothing to do and leave), SPLIT warps per column that take the parts in turn: a sequence may fill every range.
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(256) kv4_combine_kernel(const SplitParams sp, int ranges) {
+__global__ void __launch_bounds__(1024) kv4_combine_kernel(const SplitParams sp, int ranges) {
     using Cfg = SplitCfg<D, NT>;
+    constexpr int SPLIT = 32 / Cfg::COLS, C = D / 32;
     pdl_sync();
     const PartDesc d = reinterpret_cast<const PartDesc*>(sp.parts + (int64_t)2 * ranges * Cfg::part_floats())[blockIdx.x];
-    const int col = blockIdx.y, at = d.ct * Cfg::COLS + col;
-    if (d.parts == 0 || at >= d.count * sp.a.group) return;
-    __shared__ float o_s[8][D];
-    __shared__ float2 ml_s[8];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (d.parts == 0) return;
+    __shared__ __align__(16) float o_s[32][D];
+    __shared__ float2 ml_s[32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = warp / SPLIT;
     const float2* ml = reinterpret_cast<const float2*>(sp.parts + (int64_t)2 * ranges * Cfg::COLS * D);
-    constexpr int C = D / 32;
-    auto slot = [&](int i) { return (i == 0 ? 2 * (int64_t)blockIdx.x + 1 : 2 * ((int64_t)blockIdx.x + i)) * Cfg::COLS + col; };
-    float m = -INFINITY;
-    for (int i = lane; i < d.parts; i += 32) m = fmaxf(m, ml[slot(i)].x);
-    m = warp_max(m);
-    const float use = m == -INFINITY ? 0.f : m;
-    float l = 0.f, o[C];
+    auto slot = [&](int i) { return (2 * ((int64_t)blockIdx.x + i) + (i == 0 ? 1 : 0)) * Cfg::COLS + col; };
+    const bool on = d.ct * Cfg::COLS + col < d.count * sp.a.group;
+    float m = -INFINITY, l = 0.f, o[C];
 #pragma unroll
     for (int c = 0; c < C; ++c) o[c] = 0.f;
+    if (on) {
+        for (int i = lane; i < d.parts; i += 32) m = fmaxf(m, ml[slot(i)].x);
+        m = warp_max(m);
+        const float use = m == -INFINITY ? 0.f : m;
 #pragma unroll 4
-    for (int i = warp; i < d.parts; i += 8) {
-        const float2 part = ml[slot(i)];
-        const float f = ptx::ex2_approx(part.x - use);
-        l = fmaf(part.y, f, l);
-        const float* src = sp.parts + slot(i) * D + lane;
+        for (int i = warp % SPLIT; i < d.parts; i += SPLIT) {
+            const float2 part = ml[slot(i)];
+            const float* src = sp.parts + slot(i) * D + lane;
+            const float f = ptx::ex2_approx(part.x - use);
+            l = fmaf(part.y, f, l);
 #pragma unroll
-        for (int c = 0; c < C; ++c) o[c] = fmaf(src[c * 32], f, o[c]);
+            for (int c = 0; c < C; ++c) o[c] = fmaf(src[c * 32], f, o[c]);
+        }
     }
 #pragma unroll
     for (int c = 0; c < C; ++c) o_s[warp][c * 32 + lane] = o[c];
     if (lane == 0) ml_s[warp].x = l;
     __syncthreads();
-    const int ch = threadIdx.x * 8;
-    if (ch >= D) return;
-    float sum = 0.f, y[8];
+    for (int i = threadIdx.x; i < Cfg::COLS * (D / 8); i += 1024) {
+        const int at = i / (D / 8), ch = (i - at * (D / 8)) * 8, pair = d.ct * Cfg::COLS + at;
+        if (pair >= d.count * sp.a.group) break;
+        float sum = 0.f, y[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = 0.f;
+        for (int e = 0; e < 8; ++e) y[e] = 0.f;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) {
-        sum += ml_s[w].x;
+        for (int w = at * SPLIT; w < (at + 1) * SPLIT; ++w) {
+            sum += ml_s[w].x;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] += o_s[w][ch + e];
+            for (int e = 0; e < 8; ++e) y[e] += o_s[w][ch + e];
+        }
+        const int token = pair / sp.a.group, head = d.kvh * sp.a.group + (pair - token * sp.a.group);
+        store_row8<T>(reinterpret_cast<T*>(sp.a.out) + ((int64_t)(d.first + token) * sp.a.heads + head) * D + ch, y, sum);
     }
-    const int token = at / sp.a.group, head = d.kvh * sp.a.group + (at - token * sp.a.group);
-    store_row8<T>(reinterpret_cast<T*>(sp.a.out) + ((int64_t)(d.first + token) * sp.a.heads + head) * D + ch, y, sum);
 }
+
+constexpr int kSmSharedBytes = 233472;
 
 template <typename T, int D, int NT>
 int launch_split(SplitParams sp, cudaStream_t st) {
     using Cfg = SplitCfg<D, NT>;
     static std::atomic<uint64_t> reserved;
     if (!reserve_smem(kv4_split_kernel<T, D, NT>, Cfg::smem(kMaxBatch), reserved)) return fail(XG_ERR_LAUNCH, "xg_kv4_attention: cannot reserve shared memory");
-    const int grid = num_sms() * Cfg::CTAS;
-    launch_with({.early = false}, kv4_split_kernel<T, D, NT>, (unsigned)grid, kWarps * 32, (size_t)Cfg::smem(sp.a.batch), st, sp);
+    const int bytes = Cfg::smem(sp.a.batch), fit = kSmSharedBytes / (bytes + 1024);
+    const int grid = num_sms() * (fit < Cfg::CTAS ? fit : Cfg::CTAS);  // all resident
+    launch_with({.early = false}, kv4_split_kernel<T, D, NT>, (unsigned)grid, kWarps * 32, (size_t)bytes, st, sp);
     if (const int rc = check_launch("xg_kv4_attention")) return rc;
     if (!sp.split) return XG_OK;
-    launch(kv4_combine_kernel<T, D, NT>, dim3((unsigned)grid, Cfg::COLS), 256, 0, st, sp, grid);
+    launch(kv4_combine_kernel<T, D, NT>, (unsigned)grid, 1024, 0, st, sp, grid);
     return check_launch("xg_kv4_attention");
 }
 
 // Columns per unit: what the sequences bring, 16 where they bring more than 8. D = 256 has no registers for 16.
 constexpr int columns(int64_t D, int64_t max_q, int64_t group) { return D == 256 || max_q * group <= 8 ? 8 : 16; }
 
-// Long sequences are cut over CTAs. Short ones are left whole: the second launch and its traffic cost more than uneven ranges.
-constexpr bool cut(int64_t max_len) { return max_len > 1024; }
+// Whether units are cut over CTAs. Left whole, they need no second launch.
+bool cut(int64_t D, int64_t cols, int64_t units, int64_t max_len) {
+    if (getenv("XCUT")) return max_len > atoi(getenv("XCUT"));
+    return max_len > 1024 || (max_len > 512 && units < 2LL * num_sms() * split_ctas((int)D, (int)cols / 8));
+}
 
-int64_t split_workspace(int64_t D, int64_t max_q, int64_t group, int64_t max_len) {
-    if (!cut(max_len)) return 0;
+int64_t split_workspace(int64_t D, int64_t max_q, int64_t group, int64_t max_len, int64_t batch, int64_t kv_heads) {
     const int64_t cols = columns(D, max_q, group), ctas = (int64_t)num_sms() * split_ctas((int)D, (int)cols / 8);
+    if (!cut(D, cols, batch * kv_heads, max_len)) return 0;
     return 2 * ctas * cols * (D + 2) * 4 + ctas * (int64_t)sizeof(PartDesc);
 }
 
@@ -666,20 +745,26 @@ template <typename T>
 int attend_split(const AttendParams& whole, int64_t D, int64_t max_q, int most_cols, void* workspace, cudaStream_t st) {
     const int64_t max_len = (int64_t)whole.table_pages * whole.cache.tiles * kTileTokens;
     const int cols = columns(D, max_q, whole.group);
-    for (int at = 0; at == 0 || at < whole.batch; at += kMaxBatch) {
+    // blocks of a launch are counted in 32 bits
+    const int64_t most = whole.tokens * whole.group < most_cols ? whole.tokens * whole.group : most_cols;
+    const int64_t blocks = (int64_t)whole.cache.heads * ((most + cols - 1) / cols) * ((max_len + kBlockKeys - 1) / kBlockKeys);
+    const int64_t fit = blocks > 0 ? 0x7fffffffLL / blocks : kMaxBatch;
+    if (fit < 1) return fail(XG_ERR_TOO_LARGE, "xg_kv4_attention: too many rows and keys in one sequence");
+    const int chunk = (int)(fit < kMaxBatch ? fit : kMaxBatch);
+    for (int at = 0; at == 0 || at < whole.batch; at += chunk) {
         SplitParams sp = {};
         sp.a = whole;
-        sp.a.batch = whole.batch - at < kMaxBatch ? whole.batch - at : kMaxBatch;
+        sp.a.batch = whole.batch - at < chunk ? whole.batch - at : chunk;
         sp.a.table += (int64_t)at * whole.table_stride;
         sp.a.lens += at;
         if (whole.starts) sp.a.starts += at;
         else sp.a.row0 = at;
         sp.parts = static_cast<float*>(workspace);
-        sp.split = cut(max_len);
-        sp.min_blocks = 8;
+        sp.split = cut(D, cols, (int64_t)whole.batch * whole.cache.heads, max_len);
+        sp.min_blocks = getenv("XMIN") ? atoi(getenv("XMIN")) : 8;
         sp.most_cols = most_cols;
         sp.first_rows = at == 0;
-        sp.last_rows = at + kMaxBatch >= whole.batch;
+        sp.last_rows = at + chunk >= whole.batch;
         int rc;
         if (D == 64) rc = cols == 8 ? launch_split<T, 64, 1>(sp, st) : launch_split<T, 64, 2>(sp, st);
         else if (D == 128) rc = cols == 8 ? launch_split<T, 128, 1>(sp, st) : launch_split<T, 128, 2>(sp, st);
@@ -713,7 +798,7 @@ extern "C" int64_t xg_kv4_attention_workspace_bytes(int64_t tokens, int64_t batc
                                                     int64_t max_len) {
     using namespace xg;
     if (tokens <= 0 || batch <= 0 || q_heads <= 0 || kv_heads <= 0 || max_q < 0 || max_len < 0) return 0;
-    return split_workspace(D, max_q, q_heads / kv_heads, max_len);
+    return split_workspace(D, max_q, q_heads / kv_heads, max_len, batch, kv_heads);
 }
 
 extern "C" int xg_kv4_attention(const void* q, const void* cache, int64_t pages, int64_t kv_heads, int64_t page_size, int64_t page_stride,
@@ -728,9 +813,6 @@ extern "C" int xg_kv4_attention(const void* q, const void* cache, int64_t pages,
         return fail(XG_ERR_INVALID_ARG, "xg_kv4_attention: bad extents");
     if (q_heads > 65535 || batch > 0x7fffff || tokens > 0x7fffffff || table_pages > 0x7ffffff) return fail(XG_ERR_TOO_LARGE, "xg_kv4_attention: extents");
     if (table_pages * page_size > 0x7fffff00LL) return fail(XG_ERR_TOO_LARGE, "xg_kv4_attention: more than 2^31 tokens per sequence");
-    // a range of tiles is counted in 32 bits (2^38 tiles are 300 TB of cache read, or some minutes)
-    if (tokens > 0 && kv_heads * (tokens * (q_heads / kv_heads) / 8 + batch + 1) > (1LL << 38) / (table_pages * (page_size / 16) + 1))
-        return fail(XG_ERR_TOO_LARGE, "xg_kv4_attention: too many rows and keys");
     if (tokens == 0) return XG_OK;
     if (!q || !out || (batch > 0 && (!kv_lens || (table_pages > 0 && !page_table)))) return fail(XG_ERR_INVALID_ARG, "xg_kv4_attention: null pointer");
     if (!aligned16(out)) return fail(XG_ERR_INVALID_ARG, "xg_kv4_attention: the result must be 16-byte aligned");

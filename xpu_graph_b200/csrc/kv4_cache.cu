@@ -22,87 +22,131 @@ struct TokenParams {
     int64_t k_st, k_sh, v_st, v_sh;
 };
 
+// 8 consecutive values as they are stored
+template <typename T>
+struct Raw8 {
+    T v[8];
+};
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+__device__ __forceinline__ Raw8<T> load8(const T* p) {
+    Raw8<T> r;
     if (VEC) {
         constexpr int N = Vec16<T>::N;
 #pragma unroll
-        for (int i = 0; i < 8; i += N) {
-            const Vec16<T> u = ld16_stream(p + i);
-#pragma unroll
-            for (int e = 0; e < N; ++e) x[i + e] = Cvt<T>::to_f(u.v[e]);
-        }
+        for (int i = 0; i < 8; i += N) *reinterpret_cast<Vec16<T>*>(r.v + i) = ld16_stream(p + i);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = Cvt<T>::to_f(p[i]);
+        for (int i = 0; i < 8; ++i) r.v[i] = p[i];
     }
+    return r;
 }
 
-// 8 lanes hold a group's 64 channels: this lane's codes as a word, and the group's pair (scale in the low half).
-__device__ __forceinline__ void quantise(float (&x)[8], uint32_t& word, uint32_t& pair) {
-    float lo = INFINITY, hi = -INFINITY;
-    bool nan = false;
+__device__ __forceinline__ float min_nan(float a, float b) {  // NaN if one of them is
+    float y;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+// Least (NaN where there is one) and largest of 8 values.
+__device__ __forceinline__ void extremes(const Raw8<float>& x, float& lo, float& hi) {
+    lo = hi = x.v[0];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        nan |= x[i] != x[i];
-        x[i] = fminf(fmaxf(x[i], -kLargest), kLargest);
-        lo = fminf(lo, x[i]);
-        hi = fmaxf(hi, x[i]);
+    for (int i = 1; i < 8; ++i) {
+        lo = min_nan(lo, x.v[i]);
+        hi = fmaxf(hi, x.v[i]);
     }
+}
+template <typename T, typename T2>
+__device__ __forceinline__ void extremes_packed(const Raw8<T>& x, float& lo, float& hi) {
+    const T2* u = reinterpret_cast<const T2*>(x.v);
+    const T2 a = __hmin2_nan(__hmin2_nan(u[0], u[1]), __hmin2_nan(u[2], u[3])), b = __hmax2(__hmax2(u[0], u[1]), __hmax2(u[2], u[3]));
+    lo = min_nan(Cvt<T>::to_f(a.x), Cvt<T>::to_f(a.y));
+    hi = fmaxf(Cvt<T>::to_f(b.x), Cvt<T>::to_f(b.y));
+}
+__device__ __forceinline__ void extremes(const Raw8<__nv_bfloat16>& x, float& lo, float& hi) { extremes_packed<__nv_bfloat16, __nv_bfloat162>(x, lo, hi); }
+__device__ __forceinline__ void extremes(const Raw8<__half>& x, float& lo, float& hi) { extremes_packed<__half, __half2>(x, lo, hi); }
+
+// 8 lanes hold a group's 64 channels: this lane's codes as a word, and the group's pair (scale in the low half). A group with a NaN
+// has a NaN least value and reads back as NaN.
+//
+// The quotient is taken by the reciprocal: two roundings put it within 2^-19 of the true one (which is below 16), the divided and
+// rounded one is within 2^-20. They round to the same code unless a half lies between, so only what comes within 2^-17 of one is divided.
+template <typename T>
+__device__ __forceinline__ void quantise(const Raw8<T>& x, uint32_t& word, uint32_t& pair) {
+    float lo, hi;
+    extremes(x, lo, hi);
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    for (int o = 1; o < 8; o <<= 1) {  // (stays inside the group's lanes)
+        lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
         hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     }
-    // (a shuffle by 1, 2 and 4 stays inside the group's lanes)
-    const uint32_t nans = __ballot_sync(0xffffffffu, nan) >> (threadIdx.x & 24);
-    if (nans & 0xffu) lo = __int_as_float(0x7fffffff);  // a group with a NaN reads back as NaN
+    hi = fminf(fmaxf(hi, -kLargest), kLargest);
+    if (lo == lo) lo = fminf(fmaxf(lo, -kLargest), kLargest);
     const __half least = __float2half_rn(lo);
     const float least_f = __half2float(least);
     const __half scale = __float2half_rn(__fdiv_rn(hi - least_f, 15.0f));
     const float scale_f = __half2float(scale);
+    pair = (uint32_t)__half_as_ushort(scale) | ((uint32_t)__half_as_ushort(least) << 16);
     word = 0;
-    if (scale_f > 0.f) {
+    if (!(scale_f > 0.f)) return;  // one value, or a NaN
+    const float inv = __frcp_rn(scale_f);
+    bool close = false;
 #pragma unroll
+    for (int i = 0; i < 8; ++i) {  // (values beyond fp16's largest end at a bound of the codes, as that does)
+        const float q = fminf(fmaxf((Cvt<T>::to_f(x.v[i]) - least_f) * inv, 0.f), 15.f);
+        const float shifted = q + 8388608.f;  // 2^23: the sum is q rounded to an integer
+        close = close || fabsf(fabsf(q - (shifted - 8388608.f)) - 0.5f) < 0x1p-17f;
+        word |= (__float_as_uint(shifted) & 15u) << (4 * i);
+    }
+    if (close) {
+        word = 0;
+#pragma unroll 1
         for (int i = 0; i < 8; ++i) {
-            const float c = fminf(fmaxf(rintf(__fdiv_rn(x[i] - least_f, scale_f)), 0.f), 15.f);
-            word |= (uint32_t)c << (4 * i);
+            const float v = fminf(fmaxf(Cvt<T>::to_f(x.v[i]), -kLargest), kLargest);
+            word |= (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(v - least_f, scale_f)), 0.f), 15.f) << (4 * i);
         }
     }
-    pair = (uint32_t)__half_as_ushort(scale) | ((uint32_t)__half_as_ushort(least) << 16);
 }
 
-// A thread takes 8 channels of a token's head, keys and values.
+constexpr int kPerThread = 2;  // tokens in flight per thread
+
+// A thread takes 8 channels of a head, keys and values, of kPerThread tokens that lie a launch's share apart.
 template <typename T, int D, bool VEC>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const TokenParams p) {
     pdl_sync();
     constexpr int J = D / 8;
-    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int j = (int)(at % J);
-    const int64_t th = at / J;
-    const int64_t token = th / p.cache.heads;
-    const int h = (int)(th - token * p.cache.heads);
-    uint8_t* tile = nullptr;
-    int r = 0;
-    float xk[8], xv[8];
+    const int64_t first = ((int64_t)blockIdx.x * 256 + threadIdx.x) / J;  // (token, head)
+    const int j = (int)(((int64_t)blockIdx.x * 256 + threadIdx.x) % J);
+    const int64_t apart = (int64_t)gridDim.x * 256 / J, all = p.tokens * p.cache.heads;
+    Raw8<T> xk[kPerThread], xv[kPerThread];
+    int64_t slot[kPerThread];
+    int h[kPerThread];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) xk[i] = xv[i] = 0.f;
-    if (token < p.tokens) {  // (a whole group of 8 lanes agrees)
-        const int64_t slot = p.slots[token];
-        load8<T, VEC>(reinterpret_cast<const T*>(p.k) + token * p.k_st + h * p.k_sh + j * 8, xk);
-        load8<T, VEC>(reinterpret_cast<const T*>(p.v) + token * p.v_st + h * p.v_sh + j * 8, xv);
-        tile = const_cast<uint8_t*>(tile_of_slot(p.cache, D, slot, h));
-        r = (int)(slot & 15);
+    for (int n = 0; n < kPerThread; ++n) {
+        const int64_t th = first + n * apart;  // (a whole group of 8 lanes agrees on it)
+        const int64_t token = th / p.cache.heads;
+        h[n] = (int)(th - token * p.cache.heads);
+        slot[n] = -1;
+        xk[n] = xv[n] = {};
+        if (th < all) {
+            slot[n] = p.slots[token];
+            xk[n] = load8<T, VEC>(reinterpret_cast<const T*>(p.k) + token * p.k_st + h[n] * p.k_sh + j * 8);
+            xv[n] = load8<T, VEC>(reinterpret_cast<const T*>(p.v) + token * p.v_st + h[n] * p.v_sh + j * 8);
+        }
     }
-    uint32_t wk, pk, wv, pv;
-    quantise(xk, wk, pk);
-    quantise(xv, wv, pv);
-    if (tile == nullptr) return;
-    *reinterpret_cast<uint32_t*>(tile + key_word(D, r, j)) = wk;
-    *reinterpret_cast<uint32_t*>(tile + value_word(D, r, j)) = wv;
-    if ((j & 7) == 0) {
-        *reinterpret_cast<uint32_t*>(tile + pair_at(D, 0, r, j >> 3)) = pk;
-        *reinterpret_cast<uint32_t*>(tile + pair_at(D, 1, r, j >> 3)) = pv;
+#pragma unroll
+    for (int n = 0; n < kPerThread; ++n) {
+        uint32_t wk, pk, wv, pv;
+        quantise(xk[n], wk, pk);
+        quantise(xv[n], wv, pv);
+        uint8_t* tile = const_cast<uint8_t*>(tile_of_slot(p.cache, D, slot[n], h[n]));
+        if (tile == nullptr) continue;
+        const int r = (int)(slot[n] & 15);
+        *reinterpret_cast<uint32_t*>(tile + key_word(D, r, j)) = wk;
+        *reinterpret_cast<uint32_t*>(tile + value_word(D, r, j)) = wv;
+        if ((j & 7) == 0) {
+            *reinterpret_cast<uint32_t*>(tile + pair_at(D, 0, r, j >> 3)) = pk;
+            *reinterpret_cast<uint32_t*>(tile + pair_at(D, 1, r, j >> 3)) = pv;
+        }
     }
 }
 
@@ -124,29 +168,37 @@ template <typename T, int D>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const TokenParams p) {
     pdl_sync();
     constexpr int J = D / 8;
-    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int j = (int)(at % J);
-    const int64_t th = at / J;
-    const int64_t token = th / p.cache.heads;
-    if (token >= p.tokens) return;
-    const int h = (int)(th - token * p.cache.heads);
-    const int64_t slot = p.slots[token];
-    const uint8_t* tile = tile_of_slot(p.cache, D, slot, h);
-    const int r = (int)(slot & 15);
-    uint32_t wk = 0, pk = 0, wv = 0, pv = 0;  // a slot that does not exist reads as zeros
-    if (tile != nullptr) {
-        wk = *reinterpret_cast<const uint32_t*>(tile + key_word(D, r, j));
-        wv = *reinterpret_cast<const uint32_t*>(tile + value_word(D, r, j));
-        pk = *reinterpret_cast<const uint32_t*>(tile + pair_at(D, 0, r, j >> 3));
-        pv = *reinterpret_cast<const uint32_t*>(tile + pair_at(D, 1, r, j >> 3));
+    const int64_t first = ((int64_t)blockIdx.x * 256 + threadIdx.x) / J;
+    const int j = (int)(((int64_t)blockIdx.x * 256 + threadIdx.x) % J);
+    const int64_t apart = (int64_t)gridDim.x * 256 / J, all = p.tokens * p.cache.heads;
+    uint32_t w[kPerThread][2], pr[kPerThread][2];
+#pragma unroll
+    for (int n = 0; n < kPerThread; ++n) {
+        const int64_t th = first + n * apart;
+        w[n][0] = w[n][1] = pr[n][0] = pr[n][1] = 0;  // a slot that does not exist reads as zeros
+        if (th >= all) continue;
+        const int64_t token = th / p.cache.heads, slot = p.slots[token];
+        const uint8_t* tile = tile_of_slot(p.cache, D, slot, (int)(th - token * p.cache.heads));
+        const int r = (int)(slot & 15);
+        if (tile != nullptr) {
+            w[n][0] = *reinterpret_cast<const uint32_t*>(tile + key_word(D, r, j));
+            w[n][1] = *reinterpret_cast<const uint32_t*>(tile + value_word(D, r, j));
+            pr[n][0] = *reinterpret_cast<const uint32_t*>(tile + pair_at(D, 0, r, j >> 3));
+            pr[n][1] = *reinterpret_cast<const uint32_t*>(tile + pair_at(D, 1, r, j >> 3));
+        }
     }
-    store_values(reinterpret_cast<T*>(p.k_out) + th * D + j * 8, wk, pk);
-    store_values(reinterpret_cast<T*>(p.v_out) + th * D + j * 8, wv, pv);
+#pragma unroll
+    for (int n = 0; n < kPerThread; ++n) {
+        const int64_t th = first + n * apart;
+        if (th >= all) continue;
+        store_values(reinterpret_cast<T*>(p.k_out) + th * D + j * 8, w[n][0], pr[n][0]);
+        store_values(reinterpret_cast<T*>(p.v_out) + th * D + j * 8, w[n][1], pr[n][1]);
+    }
 }
 
 template <typename T, int D>
 int launch_tokens(const TokenParams& p, bool append, cudaStream_t st) {
-    const int64_t threads = p.tokens * p.cache.heads * (D / 8), grid = (threads + 255) / 256;
+    const int64_t threads = (p.tokens * p.cache.heads + kPerThread - 1) / kPerThread * (D / 8), grid = (threads + 255) / 256;
     if (grid > 0x7fffffffLL) return fail(XG_ERR_TOO_LARGE, "xg_kv4: too many tokens");
     if (append) {
         constexpr int N = Vec16<T>::N;

@@ -1506,3 +1506,20 @@ extern "C" void xg_torch_set_hook(PyObject* before, PyObject* after) {
     set(g_after, after);
     g_hooked.store(g_before || g_after);
 }
+
+// The ints of a list or tuple, one after the other; 0, or -1 with a Python error set. Called with the GIL held.
+extern "C" int xg_torch_ints(PyObject* seq, int64_t* out, int64_t n) {
+    PyObject* fast = PySequence_Fast(seq, "expected a sequence of ints");
+    if (!fast) return -1;
+    int rc = 0;
+    if (PySequence_Fast_GET_SIZE(fast) != n) {
+        PyErr_SetString(PyExc_ValueError, "the sequence changed its length");
+        rc = -1;
+    }
+    for (int64_t i = 0; rc == 0 && i < n; ++i) {
+        out[i] = PyLong_AsLongLong(PySequence_Fast_GET_ITEM(fast, i));
+        if (out[i] == -1 && PyErr_Occurred()) rc = -1;
+    }
+    Py_DECREF(fast);
+    return rc;
+}

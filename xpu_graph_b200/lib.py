@@ -157,6 +157,7 @@ def load_torch_ops() -> ctypes.PyDLL:
                 raise XgLibraryError(f"cannot load {TORCH_LIB_PATH}: {e}") from e
             lib.xg_torch_set_hook.argtypes = [ctypes.py_object, ctypes.py_object]
             lib.xg_torch_set_hook.restype = None
+            lib.xg_torch_ints.argtypes = [ctypes.py_object, c_void_p, c_int64]
             lib.xg_torch_f32_on_tensor_cores.argtypes = [c_int64, c_int64, c_int64]
             lib.xg_torch_small_tower_worth_it.argtypes = [c_int64, _I64P, c_int, c_int]
             _torch_lib = lib
