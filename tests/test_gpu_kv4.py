@@ -179,16 +179,18 @@ def _reference(q, cache, table, lens, starts, scale):
         sums = torch.einsum("hij,jhd->ihd", p, v.abs())
         err_k[lo:hi] = sums * size.transpose(0, 1)[..., None]
         groups = v.unflatten(-1, (-1, 64))
-        half_range = ((groups.amax(-1) - groups.amin(-1)) / 2)[..., None].expand_as(groups).flatten(-2)
-        err_v[lo:hi] = sums + torch.einsum("hij,jhd->ihd", p, half_range)
+        # codes times scales, as the products see them: up to the group's range, for fp16 results half of it
+        span = (groups.amax(-1) - groups.amin(-1)) * (0.5 if q.dtype == torch.float16 else 1.0)
+        err_v[lo:hi] = sums + torch.einsum("hij,jhd->ihd", p, span[..., None].expand_as(groups).flatten(-2))
     return out, err_k, err_v
 
 
 def _check_attention(got, ref, what, halves=False):
     """Scores: fp32 sums of D products, the terms' size times 2^-20 at most (16 roundings of 2^-24: the tensor core's partial sums).
     They move a probability by a factor of e^(2 error). The probability times its value's scale goes into the second product as fp16,
-    half a step of 2^-11 off, after the exponential (2^-20) and two fp32 products: that moves the value's distance from the middle of
-    its group's range, at most half the range (8/7.5 of it, as the middle is taken at code 8). What is exact beside it is an fp32 sum.
+    half a step of 2^-11 off, after the exponential (2^-20) and two fp32 products: that moves the value's distance from the least of its
+    group, at most the group's range, or for fp16 results from its middle, at most 8/7.5 of half the range. What is exact beside it is
+    an fp32 sum.
     `halves`: keys and values in fp16 too (2^-11 each of the value)."""
     out, err_k, err_v = ref
     assert got.shape == out.shape

@@ -2,7 +2,6 @@
 // ones of sequence b stands at position len_b - n_b + i and sees the keys up to its own. Heads are grouped: query head h reads kv
 // head h / (Hq / Hkv). fp32 scores, softmax and sums.
 #include "kv4_attend.cuh"
-#include <cstdlib>
 
 namespace xg {
 
@@ -27,9 +26,10 @@ using namespace kv4;
 // arithmetic.
 //   scores (16 keys x 8 columns, per group of 64 channels):  x = scale_k acc + least_k sum(q), the group's sum of q kept per column.
 //     q has a power of two per row taken out, with which bf16 fits fp16 exactly (down to 2^-29 of the row's largest).
-//   output (16 channels x 8 columns):  sum p v = sum w (code - 8) + sum p (least_v + 8 scale_v), w = p scale_v rounded to fp16 (2^-12
-//     relative). The codes go in as they are and 8 sum w comes off at the end, from a product with ones; so what the rounding moves is
-//     in proportion to half the group's range and not to its least value.
+//   output (16 channels x 8 columns):  sum p v = sum w code + sum p least_v, w = p scale_v rounded to fp16 (2^-12 relative). Rows of
+//     even channels take the whole byte (also exact) and lose the odd channel's sum at the end, which saves a mask.
+//     For fp16 results 8 sum w, from a product with ones, comes off and sum p (8 scale_v) goes in beside least_v: what the rounding
+//     moves is then in proportion to half the group's range and not to its least value (bf16 ones are 2^-9 coarse themselves).
 //     w is kept below 2^15 by the power of two that the scales have reached so far; p, up to 2^8, may be 2^29 smaller still.
 // Both that power and the maximum of a column follow their data lagging: only a step beyond them rescales the sums.
 // The codes of keys that do not exist are finite whatever they are; their scales are replaced, not multiplied away.
@@ -89,6 +89,7 @@ template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_split_kernel(const SplitParams sp) {
     using Cfg = SplitCfg<D, NT>;
     constexpr int W = D / 32, GR = D / 64;
+    constexpr bool CENTRE = std::is_same<T, __half>::value;
     const AttendParams& p = sp.a;
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t* ring = smem;
@@ -504,7 +505,7 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
 #pragma unroll
                 for (int gr = 0; gr < GR; ++gr) {
                     const float2 pa = __half22float2(vp[k][0][gr]), pb = __half22float2(vp[k][1][gr]);
-                    const float mid_a = fmaf(8.f, pa.x, pa.y), mid_b = fmaf(8.f, pb.x, pb.y);
+                    const float mid_a = CENTRE ? fmaf(8.f, pa.x, pa.y) : pa.y, mid_b = CENTRE ? fmaf(8.f, pb.x, pb.y) : pb.y;
                     uint32_t f[NT][2];  // [.][keys 0-7, 8-15]
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
@@ -523,7 +524,7 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
                         for (int c = 0; c < 2; ++c) low[nt][gr][c] += y[c] + y[2 + c];
 #pragma unroll
                         for (int r = 0; r < 2; ++r) f[nt][r] = ptx::transpose_8x8(ptx::pack2<__half>(w[2 * r], w[2 * r + 1]));
-                        ptx::mma_f16_16816(eight[nt][gr], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, f[nt][0], f[nt][1]);
+                        if (CENTRE) ptx::mma_f16_16816(eight[nt][gr], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, f[nt][0], f[nt][1]);
                     }
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
@@ -531,8 +532,9 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
                         const uint32_t u23 = __byte_perm(v[2][gr], v[3][gr], half ? 0x7632 : 0x5410);
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const uint32_t x01 = u01 >> (8 * h), x23 = u23 >> (8 * h);
-                            const uint32_t a0 = x01 & 0x000f000fu, a1 = x01 & 0x00f000f0u, a2 = x23 & 0x000f000fu, a3 = x23 & 0x00f000f0u;
+                            // (even channels' rows take the whole byte, which is exact as well: their sums lose the odd ones' at the end)
+                            const uint32_t a0 = h ? __byte_perm(u01, 0, 0x4341) : u01 & 0x00ff00ffu, a2 = h ? __byte_perm(u23, 0, 0x4341) : u23 & 0x00ff00ffu;
+                            const uint32_t a1 = a0 & 0x00f000f0u, a3 = a2 & 0x00f000f0u;
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt)
                                 ptx::mma_f16_16816(acc[nt][4 * gr + 2 * half + h], a0, a1, a2, a3, f[nt][0], f[nt][1]);
@@ -573,7 +575,7 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
                     float y[8];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        y[2 * i] = fmaf(acc[nt][4 * gr + i][c] - eight[nt][gr][c], 0x1p24f, low[nt][gr][c]);
+                        y[2 * i] = fmaf(acc[nt][4 * gr + i][c] - acc[nt][4 * gr + i][2 + c] - eight[nt][gr][c], 0x1p24f, low[nt][gr][c]);
                         y[2 * i + 1] = fmaf(acc[nt][4 * gr + i][2 + c] - 16.f * eight[nt][gr][c], 0x1p20f, low[nt][gr][c]);
                     }
                     if (whole) {
@@ -729,7 +731,6 @@ constexpr int columns(int64_t D, int64_t max_q, int64_t group) { return D == 256
 
 // Whether units are cut over CTAs. Left whole, they need no second launch.
 bool cut(int64_t D, int64_t cols, int64_t units, int64_t max_len) {
-    if (getenv("XCUT")) return max_len > atoi(getenv("XCUT"));
     return max_len > 1024 || (max_len > 512 && units < 2LL * num_sms() * split_ctas((int)D, (int)cols / 8));
 }
 
@@ -761,7 +762,7 @@ int attend_split(const AttendParams& whole, int64_t D, int64_t max_q, int most_c
         else sp.a.row0 = at;
         sp.parts = static_cast<float*>(workspace);
         sp.split = cut(D, cols, (int64_t)whole.batch * whole.cache.heads, max_len);
-        sp.min_blocks = getenv("XMIN") ? atoi(getenv("XMIN")) : 8;
+        sp.min_blocks = 8;
         sp.most_cols = most_cols;
         sp.first_rows = at == 0;
         sp.last_rows = at + chunk >= whole.batch;
