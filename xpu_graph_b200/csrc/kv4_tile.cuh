@@ -46,16 +46,16 @@ struct Cache {
 // The tile that holds `slot` (= page * page size + offset), head h; null when there is no such slot.
 __device__ __forceinline__ const uint8_t* tile_of_slot(const Cache& c, int D, int64_t slot, int h) {
     const int64_t tile = slot >> 4;
-    if (slot < 0 || tile >= c.pages * c.tiles) return nullptr;
-    const int64_t page = tile / c.tiles;
-    return c.base + page * c.page_stride + ((int64_t)h * c.tiles + (tile - page * c.tiles)) * tile_bytes(D);
+    if (slot < 0 || tile >= c.pages * c.tiles) return nullptr;  // (below 2^32: check_cache)
+    const uint32_t page = (uint32_t)tile / (uint32_t)c.tiles, in_page = (uint32_t)tile - page * (uint32_t)c.tiles;
+    return c.base + page * c.page_stride + ((int64_t)h * c.tiles + in_page) * tile_bytes(D);
 }
 
 inline int check_cache(const char* who, const void* base, int64_t pages, int64_t heads, int64_t page_size, int64_t page_stride, int64_t D) {
     if (D != 64 && D != 128 && D != 256) return fail(XG_ERR_UNSUPPORTED, "%s: head_dim %lld is not 64, 128 or 256", who, (long long)D);
     if (pages < 0 || heads <= 0 || page_size <= 0 || page_size % kTileTokens != 0)
         return fail(XG_ERR_INVALID_ARG, "%s: bad cache extents (a page holds a multiple of 16 tokens)", who);
-    if (heads > 65535 || page_size > (1 << 20) || pages > (1LL << 40)) return fail(XG_ERR_TOO_LARGE, "%s: cache extents", who);
+    if (heads > 65535 || page_size > (1 << 20) || pages > 0xffffffffLL / (page_size / kTileTokens)) return fail(XG_ERR_TOO_LARGE, "%s: cache extents", who);
     if (page_stride % 16 != 0 || (pages > 1 && page_stride < heads * (page_size / 16) * tile_bytes((int)D)) || !aligned16(base))
         return fail(XG_ERR_INVALID_ARG, "%s: pages must start on 16-byte boundaries and not overlap", who);
     if (pages > 0 && !base) return fail(XG_ERR_INVALID_ARG, "%s: null pointer", who);
