@@ -233,6 +233,8 @@ ATTEND = [  # d, kv heads, group, page, lens, new tokens (None: one each, withou
     (128, 1, 8, 32, [1500], [300]),
     (128, 4, 3, 16, [257, 77, 500], [86, 77, 85]),
     (64, 2, 5, 128, [3000, 64], [40, 64]),
+    (128, 1, 4, 64, [6000, 700, 90], [100, 90, 80]),  # few rows, many keys
+    (64, 2, 1, 32, [2500], [200]),
     (128, 1, 1, 16, [70, 0, 100], [90, 66, 130]),
     (256, 1, 2, 32, [150], [150]),
 ]

@@ -740,7 +740,9 @@ int64_t split_workspace(int64_t D, int64_t max_q, int64_t group, int64_t max_len
     return 2 * ctas * cols * (D + 2) * 4 + ctas * (int64_t)sizeof(PartDesc);
 }
 
+// Sequences with more columns (new token, head of the group) than this go to the tensor-memory kernel.
 constexpr int kMostStreamed = 64;
+constexpr bool in_tiles(int64_t D, int64_t max_q, int64_t group) { return D != 256 && max_q * group > kMostStreamed; }
 
 template <typename T>
 int attend_split(const AttendParams& whole, int64_t D, int64_t max_q, int most_cols, void* workspace, cudaStream_t st) {
@@ -799,7 +801,9 @@ extern "C" int64_t xg_kv4_attention_workspace_bytes(int64_t tokens, int64_t batc
                                                     int64_t max_len) {
     using namespace xg;
     if (tokens <= 0 || batch <= 0 || q_heads <= 0 || kv_heads <= 0 || max_q < 0 || max_len < 0) return 0;
-    return split_workspace(D, max_q, q_heads / kv_heads, max_len, batch, kv_heads);
+    const int64_t group = q_heads / kv_heads, streamed = split_workspace(D, max_q, group, max_len, batch, kv_heads);
+    const int64_t tiles = in_tiles(D, max_q, group) ? prefill_workspace(tokens, batch, group, kv_heads, D, max_len) : 0;
+    return streamed > tiles ? streamed : tiles;  // (used one after the other)
 }
 
 extern "C" int xg_kv4_attention(const void* q, const void* cache, int64_t pages, int64_t kv_heads, int64_t page_size, int64_t page_stride,
@@ -828,8 +832,8 @@ extern "C" int xg_kv4_attention(const void* q, const void* cache, int64_t pages,
         return fail(XG_ERR_INVALID_ARG, "xg_kv4_attention: needs %lld bytes of 16-byte aligned workspace", (long long)need);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     // Sequences with many columns go to the tensor-memory kernel, where there may be any; the others to the streaming one.
-    const bool tiles = D != 256 && batch > 0 && max_q * p.group > kMostStreamed;
+    const bool tiles = batch > 0 && in_tiles(D, max_q, p.group);
     const int most = tiles ? kMostStreamed : 0x7fffffff;
     const int rc = dtype == XG_BF16 ? attend_split<__nv_bfloat16>(p, D, max_q, most, workspace, st) : attend_split<__half>(p, D, max_q, most, workspace, st);
-    return rc != XG_OK || !tiles ? rc : attend_prefill(p, D, dtype, most, st);
+    return rc != XG_OK || !tiles ? rc : attend_prefill(p, D, dtype, most, workspace, st);
 }

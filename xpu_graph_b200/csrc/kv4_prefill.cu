@@ -38,17 +38,26 @@ struct PreCfg {
 
 struct Unit {
     int on, b, kvh, rt;  // rt: which 256 rows
-    int first, count, len;
+    int first, count, len, pad;
 };
 
-// 8 codes as fp16 values, in channel order
+// Keys shared out over several CTAs: their parts, unnormalised. Rows of all parts, (maximum, sum) pairs, then a Unit per unit.
+struct Parts {
+    float* rows;  // [units][splits][256][D]
+    float2* ml;   // [units][splits][256]
+    Unit* unit;   // [units]
+    int splits;   // 1: none of this
+};
+
+// 8 codes as fp16 values, in the order 0 4 1 5 2 6 3 7, in which masks find them: q lies in that order too, and the output's columns
+// are put right when they leave. `scale` and `least` in both halves.
 __device__ __forceinline__ uint4 unpack8(uint32_t w, __half2 scale, __half2 least) {
     uint32_t out[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        // byte k in both halves; its low code becomes 1024 + n in the low half, its high code 64 + n in the high half
-        const uint32_t y = (__byte_perm(w, 0, 0x4040 + k * 0x0101) & 0x00f0000fu) | 0x54006400u;
-        const __half2 n = __hsub2(*reinterpret_cast<const __half2*>(&y), __halves2half2(__ushort_as_half(0x6400), __ushort_as_half(0x5400)));
+        // a code in bits 0-3 of a half becomes 1024 + n, one in bits 4-7 64 + n
+        const uint32_t y = ((w >> (8 * (k / 2))) & ((k & 1) ? 0x00f000f0u : 0x000f000fu)) | ((k & 1) ? 0x54005400u : 0x64006400u);
+        const __half2 n = __hsub2(*reinterpret_cast<const __half2*>(&y), __half2half2(__ushort_as_half((k & 1) ? 0x5400 : 0x6400)));
         const __half2 v = __hfma2(n, scale, least);
         out[k] = *reinterpret_cast<const uint32_t*>(&v);
     }
@@ -56,7 +65,7 @@ __device__ __forceinline__ uint4 unpack8(uint32_t w, __half2 scale, __half2 leas
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const AttendParams p, int beyond) {
+__global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const AttendParams p, int beyond, const Parts parts) {
     using Cfg = PreCfg<D>;
     constexpr int W = D / 32, GR = D / 64;
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -128,16 +137,16 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
                 const int v = __shfl_up_sync(0xffffffffu, inc, o);
                 if (lane >= o) inc += v;
             }
-            const int at = (int)blockIdx.x - base;
+            const int at = (int)blockIdx.x / parts.splits - base;
             if (at >= inc - w && at < inc) {
                 const int off = at - (inc - w), tiles = w / p.cache.heads;
-                u = {1, b, off % p.cache.heads, tiles - 1 - off / p.cache.heads, (int)s.first, s.count, (int)s.len};
+                u = {1, b, off % p.cache.heads, tiles - 1 - off / p.cache.heads, (int)s.first, s.count, (int)s.len, 0};
                 *unit = u;
             }
             if (__any_sync(0xffffffffu, u.on)) break;
             base += __shfl_sync(0xffffffffu, inc, 31);
         }
-        if (!__any_sync(0xffffffffu, u.on) && lane == 0) unit->on = 0;
+        if (!__any_sync(0xffffffffu, u.on) && lane == 0) *unit = {};
     }
     ptx::tc_fence_before();
     __syncthreads();
@@ -153,7 +162,11 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
         const int seen = u.len - u.count + (min(rows, lo + PM) - 1) / p.group + 1;
         return seen > 0 ? (seen + PN - 1) / PN : 0;
     };
-    const int nblk0 = blocks_of(0), nblk1 = blocks_of(1), nblk = max(nblk0, nblk1);
+    // blocks j0 .. of this CTA; every role counts them from 0
+    const int all_blocks = max(blocks_of(0), blocks_of(1)), split = (int)blockIdx.x % parts.splits;
+    const int j0 = (int)((int64_t)all_blocks * split / parts.splits), nblk = (int)((int64_t)all_blocks * (split + 1) / parts.splits) - j0;
+    const int nblk0 = min(nblk, max(0, blocks_of(0) - j0)), nblk1 = min(nblk, max(0, blocks_of(1) - j0));
+    if (parts.splits > 1 && split == 0 && threadIdx.x == 0) parts.unit[blockIdx.x / parts.splits] = u;
 
     if (warp < kUnpackWarps) {
         // ------------------------------ unpacking ---------------------------------
@@ -164,7 +177,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
         auto issue = [&](int j) {  // this warp's tile of block j
             if (j >= nblk) return;
             if ((j & 31) == 0) {
-                const int tile = (j + lane) * kUnpackWarps + warp;
+                const int tile = (j0 + j + lane) * kUnpackWarps + warp;
                 addr = tile * kTileTokens < u.len ? tile_of_token(p, u.b, u.kvh, tile, Cfg::TILE) : 0;
             }
             const int64_t from = __shfl_sync(0xffffffffu, addr, j & 31);
@@ -190,7 +203,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
             if (!__all_sync(0xffffffffu, ptx::mbar_wait_bounded(&my_full[stage], (uint32_t)(j / kRing) & 1u, abort_flag))) { ok = false; break; }
             const uint8_t* tile = my_ring + stage * Cfg::TILE;
             const int hole = my_hole[stage];
-            const int there = hole ? 0 : u.len - (j * kUnpackWarps + warp) * kTileTokens;  // tokens of the tile that exist
+            const int there = hole ? 0 : u.len - ((j0 + j) * kUnpackWarps + warp) * kTileTokens;  // tokens of the tile that exist
             if (!__all_sync(0xffffffffu, ptx::mbar_wait_bounded(&k_empty[buf], ph ^ 1u, abort_flag))) { ok = false; break; }
             if (lane == 0) holes[(j & 3) * kUnpackWarps + warp] = hole;
             {
@@ -203,11 +216,11 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
                     load_words<W>(tile + r * (D / 2) + kt * (D / 8), words);
                     load_pairs<GR>(tile + pair_at(D, 0, r, 0), pairs);
 #pragma unroll
-                    for (int w = 0; w < W; ++w) {
-                        const __half2 pair = r < there ? pairs[w / 2] : zero;
-                        const int c = (4 * w + kt) & 7;
-                        ptx::st_shared_v4(base + (uint32_t)((w / 2) * (PN * 128) + r * 128 + ((c ^ (r & 7)) << 4)),
-                                          unpack8(words[w], __low2half2(pair), __high2half2(pair)));
+                    for (int gr = 0; gr < GR; ++gr) {
+                        const __half2 pair = r < there ? pairs[gr] : zero, scale = __low2half2(pair), least = __high2half2(pair);
+#pragma unroll
+                        for (int w = 0; w < 2; ++w)  // chunks 4 w + kt
+                            ptx::st_shared_v4(base + (uint32_t)(gr * (PN * 128) + r * 128 + (((4 * w + kt) ^ (r & 7)) << 4)), unpack8(words[2 * gr + w], scale, least));
                     }
                 }
             }
@@ -339,7 +352,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
                 const T* e8 = reinterpret_cast<const T*>(&raw[c]);
                 uint32_t w[4];
 #pragma unroll
-                for (int x = 0; x < 4; ++x) w[x] = ptx::pack2<__half>(Cvt<T>::to_f(e8[2 * x]) * down, Cvt<T>::to_f(e8[2 * x + 1]) * down);
+                for (int x = 0; x < 4; ++x) w[x] = ptx::pack2<__half>(Cvt<T>::to_f(e8[x]) * down, Cvt<T>::to_f(e8[x + 4]) * down);  // (unpack8's order)
                 ptx::st_shared_v4(base + (uint32_t)((c >> 3) * (PM * 128) + (((c & 7) ^ (r_in_tile & 7)) << 4)), make_uint4(w[0], w[1], w[2], w[3]));
             }
             ptx::fence_proxy_async();
@@ -354,7 +367,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
             if (!__all_sync(0xffffffffu, ptx::mbar_wait_bounded(&s_full[2 * i + buf], (uint32_t)(j >> 1) & 1u, abort_flag))) { ok = false; break; }
             ptx::tc_fence_after();
             const uint32_t s_taddr = tmem_base + lane_field + (uint32_t)((2 * i + buf) * PN);
-            const int visible = limit - j * PN;  // columns of this block that the row sees
+            const int visible = limit - (j0 + j) * PN;  // columns of this block that the row sees
             int hole = 0;
 #pragma unroll
             for (int w = 0; w < kUnpackWarps; ++w) hole |= (holes[(j & 3) * kUnpackWarps + w] != 0) << w;
@@ -447,7 +460,24 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
             ptx::mbar_arrive(&p_full[2 * i + buf]);
         }
         if (ok && n > 0) ok = __all_sync(0xffffffffu, ptx::mbar_wait_bounded(&o_full[i], 0, abort_flag)) != 0;
-        if (ok && u.on && lo + quad * 32 < rows) {
+        if (ok && parts.splits > 1 && there) {
+            ptx::tc_fence_after();
+            const int64_t at = (int64_t)blockIdx.x * (2 * PM) + i * PM + r_in_tile;
+            parts.ml[at] = make_float2(m_run, l_run);
+        }
+        if (ok && parts.splits > 1 && u.on && lo + quad * 32 < rows) {
+            const int64_t at = (int64_t)blockIdx.x * (2 * PM) + i * PM + r_in_tile;
+#pragma unroll 1
+            for (int c = 0; c < D / 32 && n > 0; ++c) {
+                uint32_t o[32];
+                ptx::tmem_ld_32x32(o_taddr + (uint32_t)(c * 32), o);
+                ptx::tmem_ld_wait();
+                if (!there) continue;
+#pragma unroll
+                for (int x = 0; x < 32; x += 4) *reinterpret_cast<uint4*>(parts.rows + at * D + c * 32 + x) = make_uint4(o[x], o[x + 1], o[x + 2], o[x + 3]);
+            }
+            ptx::tc_fence_before();
+        } else if (ok && u.on && lo + quad * 32 < rows) {
             ptx::tc_fence_after();
             const float inv_l = l_run > 0.f || l_run != l_run ? 1.0f / l_run : 0.f;
             // rows leave through a slab of shared memory (this tile's q, which no product reads any more), so that stores are whole lines
@@ -467,7 +497,10 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
                 for (int t4 = 0; t4 < 4; ++t4) {
                     uint32_t w[4];
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) w[x] = ptx::pack2<T>(__uint_as_float(o[t4 * 8 + 2 * x]) * inv_l, __uint_as_float(o[t4 * 8 + 2 * x + 1]) * inv_l);
+                    for (int x = 0; x < 4; ++x) {  // channels 2 x, 2 x + 1 (unpack8's order)
+                        const int at = t4 * 8 + 4 * (x & 1) + (x >> 1);
+                        w[x] = ptx::pack2<T>(__uint_as_float(o[at]) * inv_l, __uint_as_float(o[at + 2]) * inv_l);
+                    }
                     const int at = (c & 1) * 4 + t4;
                     ptx::st_shared_v4(slab + (uint32_t)(lane * 128 + ((at ^ (lane & 7)) << 4)), make_uint4(w[0], w[1], w[2], w[3]));
                 }
@@ -498,23 +531,83 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
     }
 }
 
+// out = sum 2^(m_i - m) O_i / sum 2^(m_i - m) l_i over a row's parts, a warp per row. Parts that saw no key have written no row.
 template <typename T, int D>
-int launch_prefill(const AttendParams& p, int beyond, cudaStream_t st) {
+__global__ void __launch_bounds__(256) kv4_prefill_combine_kernel(const AttendParams p, const Parts parts) {
+    pdl_sync();
+    const Unit u = parts.unit[blockIdx.x];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int in_unit = blockIdx.y * 8 + warp, row = u.rt * 2 * PM + in_unit;
+    if (!u.on || row >= u.count * p.group) return;
+    auto at = [&](int i) { return ((int64_t)blockIdx.x * parts.splits + i) * (2 * PM) + in_unit; };
+    float m = -INFINITY;
+    for (int i = lane; i < parts.splits; i += 32) m = fmaxf(m, parts.ml[at(i)].x);
+    m = warp_max(m);
+    const float use = m == -INFINITY ? 0.f : m;
+    constexpr int C = D / 32;  // columns C lane ..
+    float l = 0.f, o[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) o[c] = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < parts.splits; ++i) {
+        const float2 part = parts.ml[at(i)];
+        if (part.x == -INFINITY && part.y == 0.f) continue;
+        const float f = ptx::ex2_approx(part.x - use);
+        l = fmaf(part.y, f, l);
+#pragma unroll
+        for (int c = 0; c < C; ++c) o[c] = fmaf(parts.rows[at(i) * D + c * 32 + lane], f, o[c]);
+    }
+    const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
+    const int token = row / p.group, head = u.kvh * p.group + (row - token * p.group);
+    T* out = reinterpret_cast<T*>(p.out) + ((int64_t)(u.first + token) * p.heads + head) * D;
+    // column x of 8 is channel 4 (x & 1) + x / 2 (unpack8's order)
+    const int ch = (lane & ~7) + 4 * (lane & 1) + ((lane & 7) >> 1);
+#pragma unroll
+    for (int c = 0; c < C; ++c) out[c * 32 + ch] = Cvt<T>::from_f(o[c] * inv);
+}
+
+// The most units there can be, and over how many CTAs each one's keys are shared out: as many as fill the chip once, 512 keys or more each.
+int64_t most_units(int64_t tokens, int64_t batch, int64_t group, int64_t heads) { return (tokens * group + batch * (2 * PM - 1)) / (2 * PM) * heads; }
+int key_splits(int64_t units, int64_t max_len) {
+    int64_t n = num_sms() / (units > 0 ? units : 1);
+    if (n > max_len / 512) n = max_len / 512;
+    return (int)(n < 1 ? 1 : n);
+}
+
+template <typename T, int D>
+int launch_prefill(const AttendParams& p, int beyond, void* workspace, cudaStream_t st) {
     using Cfg = PreCfg<D>;
     static std::atomic<uint64_t> reserved;
     if (!reserve_smem(kv4_prefill_kernel<T, D>, Cfg::SMEM, reserved)) return fail(XG_ERR_LAUNCH, "xg_kv4_attention: cannot reserve shared memory");
     // at least as many CTAs as there are units; those behind the last one return at once
-    const int64_t grid = (p.tokens * p.group / (2 * PM) + p.batch) * p.cache.heads;
-    if (grid > 0x7fffffffLL) return fail(XG_ERR_TOO_LARGE, "xg_kv4_attention: too many rows");
-    launch_with({.early = false}, kv4_prefill_kernel<T, D>, (unsigned)grid, kPrefillThreads, Cfg::SMEM, st, p, beyond);
+    const int64_t units = most_units(p.tokens, p.batch, p.group, p.cache.heads);
+    Parts parts = {};
+    parts.splits = key_splits(units, (int64_t)p.table_pages * p.cache.tiles * kTileTokens);
+    if (units * parts.splits > 0x7fffffffLL) return fail(XG_ERR_TOO_LARGE, "xg_kv4_attention: too many rows");
+    if (parts.splits > 1) {
+        const int64_t rows = units * parts.splits * 2 * PM;
+        parts.rows = static_cast<float*>(workspace);
+        parts.ml = reinterpret_cast<float2*>(parts.rows + rows * D);
+        parts.unit = reinterpret_cast<Unit*>(parts.ml + rows);
+    }
+    launch_with({.early = false}, kv4_prefill_kernel<T, D>, (unsigned)(units * parts.splits), kPrefillThreads, Cfg::SMEM, st, p, beyond, parts);
+    if (const int rc = check_launch("xg_kv4_attention")) return rc;
+    if (parts.splits == 1) return XG_OK;
+    launch(kv4_prefill_combine_kernel<T, D>, dim3((unsigned)units, 2 * PM / 8), 256, 0, st, p, parts);
     return check_launch("xg_kv4_attention");
 }
 
 }  // namespace
 
-int attend_prefill(const AttendParams& p, int64_t D, int dtype, int beyond, cudaStream_t st) {
-    if (dtype == XG_BF16) return D == 64 ? launch_prefill<__nv_bfloat16, 64>(p, beyond, st) : launch_prefill<__nv_bfloat16, 128>(p, beyond, st);
-    return D == 64 ? launch_prefill<__half, 64>(p, beyond, st) : launch_prefill<__half, 128>(p, beyond, st);
+int64_t prefill_workspace(int64_t tokens, int64_t batch, int64_t group, int64_t heads, int64_t D, int64_t max_len) {
+    const int64_t units = most_units(tokens, batch, group, heads);
+    const int splits = key_splits(units, max_len);
+    return splits == 1 ? 0 : units * splits * 2 * PM * (D + 2) * 4 + units * (int64_t)sizeof(Unit);
+}
+
+int attend_prefill(const AttendParams& p, int64_t D, int dtype, int beyond, void* workspace, cudaStream_t st) {
+    if (dtype == XG_BF16) return D == 64 ? launch_prefill<__nv_bfloat16, 64>(p, beyond, workspace, st) : launch_prefill<__nv_bfloat16, 128>(p, beyond, workspace, st);
+    return D == 64 ? launch_prefill<__half, 64>(p, beyond, workspace, st) : launch_prefill<__half, 128>(p, beyond, workspace, st);
 }
 
 int read_kv4_prefill_status(unsigned int* host_out, int reset) {
