@@ -14,7 +14,7 @@ def _quantised(x):
     """Values, codes, scales and least values of [..., d], step by step as they are defined, in fp32 on the CPU."""
     y = x.detach().cpu().float().clamp(-65504.0, 65504.0).unflatten(-1, (-1, 64))
     least = y.amin(-1).half()  # (amin keeps NaN)
-    scale = ((y.amax(-1) - least.float()) / 15.0).half()
+    scale = ((y.amax(-1) - least.float()) * torch.tensor(1 / 15)).half()
     code = ((y - least.float()[..., None]) / scale.float()[..., None]).round().clamp(0, 15)
     code = torch.where(scale[..., None] > 0, code, torch.zeros(()))
     return (code * scale.float()[..., None] + least.float()[..., None]).flatten(-2).to(x.dtype), code.flatten(-2), scale, least
@@ -179,18 +179,16 @@ def _reference(q, cache, table, lens, starts, scale):
         sums = torch.einsum("hij,jhd->ihd", p, v.abs())
         err_k[lo:hi] = sums * size.transpose(0, 1)[..., None]
         groups = v.unflatten(-1, (-1, 64))
-        # codes times scales, as the products see them: up to the group's range, for fp16 results half of it
-        span = (groups.amax(-1) - groups.amin(-1)) * (0.5 if q.dtype == torch.float16 else 1.0)
-        err_v[lo:hi] = sums + torch.einsum("hij,jhd->ihd", p, span[..., None].expand_as(groups).flatten(-2))
+        half_range = ((groups.amax(-1) - groups.amin(-1)) / 2)[..., None].expand_as(groups).flatten(-2)
+        err_v[lo:hi] = sums + torch.einsum("hij,jhd->ihd", p, half_range)
     return out, err_k, err_v
 
 
 def _check_attention(got, ref, what, halves=False):
     """Scores: fp32 sums of D products, the terms' size times 2^-20 at most (16 roundings of 2^-24: the tensor core's partial sums).
     They move a probability by a factor of e^(2 error). The probability times its value's scale goes into the second product as fp16,
-    half a step of 2^-11 off, after the exponential (2^-20) and two fp32 products: that moves the value's distance from the least of its
-    group, at most the group's range, or for fp16 results from its middle, at most 8/7.5 of half the range. What is exact beside it is
-    an fp32 sum.
+    half a step of 2^-11 off, after the exponential (2^-20) and two fp32 products: that moves the value's distance from the middle of
+    its group's range, at most half the range (8/7.5 of it, as the middle is taken at code 8). What is exact beside it is an fp32 sum.
     `halves`: keys and values in fp16 too (2^-11 each of the value)."""
     out, err_k, err_v = ref
     assert got.shape == out.shape
@@ -237,6 +235,7 @@ ATTEND = [  # d, kv heads, group, page, lens, new tokens (None: one each, withou
     (64, 2, 1, 32, [2500], [200]),
     (128, 1, 1, 16, [70, 0, 100], [90, 66, 130]),
     (256, 1, 2, 32, [150], [150]),
+    (256, 2, 3, 64, [2000, 70, 300], [40, 2, 90]),
 ]
 
 
@@ -344,6 +343,24 @@ def test_attention_is_repeatable_and_any_hint_will_do(cuda_device):
     assert torch.equal(one, ops.kv4_attention(q, cache, table, n, at, 3, 0.1))
     for hint in (0, 1, 100000):
         _check_attention(ops.kv4_attention(q, cache, table, n, at, hint, 0.1), _reference(q, cache, table, lens, starts, 0.1), f"hint {hint}", halves=hint > 8)
+
+
+def test_a_flat_average_over_a_long_history(cuda_device):
+    """131072 keys of equal weight: the average is 1 / 360 of the values, where a bias of the sums would show."""
+    from xpu_graph_b200 import ops
+
+    n, g = 131072, torch.Generator(cuda_device).manual_seed(0)
+    cache = torch.zeros(n // 64, 1, 4, 18 * 128, dtype=torch.uint8, device=cuda_device)
+    v = torch.randn(n, 1, 128, generator=g, device=cuda_device)
+    ops.kv4_append(cache, v, v, torch.arange(n, device=cuda_device))
+    want = ops.kv4_read(cache, torch.arange(n, device=cuda_device), torch.float32)[1].double().mean(0)
+    table = torch.arange(n // 64, device=cuda_device)[None]
+    for rows in (1, 60):
+        q = torch.zeros(rows, 1, 128, device=cuda_device).half()
+        got = ops.kv4_attention(q, cache, table, torch.tensor([n + rows - 1], device=cuda_device).clamp(max=n), torch.tensor([0, rows], device=cuda_device), rows, 1.0)[-1]
+        # independent roundings of 2^-11 at most of values of 1 around a mean of 0, over 360: below 2^-11 of the mean's size, twice for
+        # keys in fp16; the result's own 2^-11; sums of 128 keys in fp32 with 2^-24 of up to 15 a step: below 2^-9 together
+        assert ((got.double() - want).norm() / want.norm()).item() < 2.0 ** -9
 
 
 # ---- pages -----------------------------------------------------------------------------------------

@@ -26,10 +26,12 @@ using namespace kv4;
 // arithmetic.
 //   scores (16 keys x 8 columns, per group of 64 channels):  x = scale_k acc + least_k sum(q), the group's sum of q kept per column.
 //     q has a power of two per row taken out, with which bf16 fits fp16 exactly (down to 2^-29 of the row's largest).
-//   output (16 channels x 8 columns):  sum p v = sum w code + sum p least_v, w = p scale_v rounded to fp16 (2^-12 relative). Rows of
-//     even channels take the whole byte (also exact) and lose the odd channel's sum at the end, which saves a mask.
-//     For fp16 results 8 sum w, from a product with ones, comes off and sum p (8 scale_v) goes in beside least_v: what the rounding
-//     moves is then in proportion to half the group's range and not to its least value (bf16 ones are 2^-9 coarse themselves).
+//   output (16 channels x 8 columns):  sum p v = sum w (code - 8) + sum p (least_v + 8 scale_v), w = p scale_v rounded to fp16 (2^-12
+//     relative). The codes go in as they are; 8 sum w, from a product with ones, comes off every 256 keys, before the sums have
+//     grown so far that what the tensor core cuts off below 2^-24 of them is a bias (a flat average over 131072 keys would be 3 % off).
+//     It cuts by the operands' exponents, which subnormals do not have: a code 2^-20 loses four bits less than one 2^-24. Where that
+//     shows, in fp16 results, both codes of a byte go in as 2^-20 (131072 keys: 0.00036 of the result, then 0.00030; 0.00021 is its
+//     own rounding), for one operation of the FMA pipe per register.
 //     w is kept below 2^15 by the power of two that the scales have reached so far; p, up to 2^8, may be 2^29 smaller still.
 // Both that power and the maximum of a column follow their data lagging: only a step beyond them rescales the sums.
 // The codes of keys that do not exist are finite whatever they are; their scales are replaced, not multiplied away.
@@ -89,7 +91,10 @@ template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_split_kernel(const SplitParams sp) {
     using Cfg = SplitCfg<D, NT>;
     constexpr int W = D / 32, GR = D / 64;
-    constexpr bool CENTRE = std::is_same<T, __half>::value;
+    // fp16 results: the even channels' value codes are moved up to the odd ones' place, see above
+    constexpr bool FINE = std::is_same<T, __half>::value;
+    constexpr float kEven = FINE ? 0x1p20f : 0x1p24f, kOdd = 0x1p20f, kOddEight = FINE ? 1.f : 16.f;
+    constexpr uint32_t kEight = FINE ? 0x00800080u : 0x00080008u;
     const AttendParams& p = sp.a;
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t* ring = smem;
@@ -505,7 +510,7 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
 #pragma unroll
                 for (int gr = 0; gr < GR; ++gr) {
                     const float2 pa = __half22float2(vp[k][0][gr]), pb = __half22float2(vp[k][1][gr]);
-                    const float mid_a = CENTRE ? fmaf(8.f, pa.x, pa.y) : pa.y, mid_b = CENTRE ? fmaf(8.f, pb.x, pb.y) : pb.y;
+                    const float mid_a = fmaf(8.f, pa.x, pa.y), mid_b = fmaf(8.f, pb.x, pb.y);
                     uint32_t f[NT][2];  // [.][keys 0-7, 8-15]
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
@@ -524,7 +529,7 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
                         for (int c = 0; c < 2; ++c) low[nt][gr][c] += y[c] + y[2 + c];
 #pragma unroll
                         for (int r = 0; r < 2; ++r) f[nt][r] = ptx::transpose_8x8(ptx::pack2<__half>(w[2 * r], w[2 * r + 1]));
-                        if (CENTRE) ptx::mma_f16_16816(eight[nt][gr], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, f[nt][0], f[nt][1]);
+                        ptx::mma_f16_16816(eight[nt][gr], kEight, kEight, kEight, kEight, f[nt][0], f[nt][1]);
                     }
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
@@ -532,9 +537,9 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
                         const uint32_t u23 = __byte_perm(v[2][gr], v[3][gr], half ? 0x7632 : 0x5410);
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            // (even channels' rows take the whole byte, which is exact as well: their sums lose the odd ones' at the end)
-                            const uint32_t a0 = h ? __byte_perm(u01, 0, 0x4341) : u01 & 0x00ff00ffu, a2 = h ? __byte_perm(u23, 0, 0x4341) : u23 & 0x00ff00ffu;
-                            const uint32_t a1 = a0 & 0x00f000f0u, a3 = a2 & 0x00f000f0u;
+                            const uint32_t x01 = u01 >> (8 * h), x23 = u23 >> (8 * h);
+                            const uint32_t a0 = FINE ? (x01 * 16u) & 0x00f000f0u : x01 & 0x000f000fu, a2 = FINE ? (x23 * 16u) & 0x00f000f0u : x23 & 0x000f000fu;
+                            const uint32_t a1 = x01 & 0x00f000f0u, a3 = x23 & 0x00f000f0u;
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt)
                                 ptx::mma_f16_16816(acc[nt][4 * gr + 2 * half + h], a0, a1, a2, a3, f[nt][0], f[nt][1]);
@@ -545,6 +550,21 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
             }
             __syncwarp();  // every lane has read the stage
             issue(done + Cfg::STAGES, stage);
+            if ((done & 7) == 7) {  // 8 sum w comes off
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int gr = 0; gr < GR; ++gr)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                            for (int i = 4 * gr; i < 4 * gr + 4; ++i) {
+                                acc[nt][i][c] -= eight[nt][gr][c];
+                                acc[nt][i][2 + c] = fmaf(-kOddEight, eight[nt][gr][c], acc[nt][i][2 + c]);
+                            }
+                            eight[nt][gr][c] = eight[nt][gr][2 + c] = 0.f;
+                        }
+            }
             if (++stage == Cfg::STAGES) {
                 stage = 0;
                 phase ^= 1u;
@@ -575,8 +595,8 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
                     float y[8];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        y[2 * i] = fmaf(acc[nt][4 * gr + i][c] - acc[nt][4 * gr + i][2 + c] - eight[nt][gr][c], 0x1p24f, low[nt][gr][c]);
-                        y[2 * i + 1] = fmaf(acc[nt][4 * gr + i][2 + c] - 16.f * eight[nt][gr][c], 0x1p20f, low[nt][gr][c]);
+                        y[2 * i] = fmaf(acc[nt][4 * gr + i][c] - eight[nt][gr][c], kEven, low[nt][gr][c]);
+                        y[2 * i + 1] = fmaf(acc[nt][4 * gr + i][2 + c] - kOddEight * eight[nt][gr][c], kOdd, low[nt][gr][c]);
                     }
                     if (whole) {
                         if (pair < count * p.group) store_row8<T>(out + 64 * gr, y, l[nt][c]);
@@ -741,8 +761,10 @@ int64_t split_workspace(int64_t D, int64_t max_q, int64_t group, int64_t max_len
 }
 
 // Sequences with more columns (new token, head of the group) than this go to the tensor-memory kernel.
-constexpr int kMostStreamed = 64;
-constexpr bool in_tiles(int64_t D, int64_t max_q, int64_t group) { return D != 256 && max_q * group > kMostStreamed; }
+// Streaming unpacks the keys once per 16 columns, the other once per 256: (us, streamed / tiles, 32/8 heads of 128) 8 sequences of 4096,
+// 48 columns 54 / 57; of 8192, 64 columns 111 / 94; of 4096, 120 columns 109 / 90; 1 of 8192, 64 columns 31 / 32.
+constexpr int kMostStreamed = 48;
+constexpr bool in_tiles(int64_t max_q, int64_t group) { return max_q * group > kMostStreamed; }
 
 template <typename T>
 int attend_split(const AttendParams& whole, int64_t D, int64_t max_q, int most_cols, void* workspace, cudaStream_t st) {
@@ -802,7 +824,7 @@ extern "C" int64_t xg_kv4_attention_workspace_bytes(int64_t tokens, int64_t batc
     using namespace xg;
     if (tokens <= 0 || batch <= 0 || q_heads <= 0 || kv_heads <= 0 || max_q < 0 || max_len < 0) return 0;
     const int64_t group = q_heads / kv_heads, streamed = split_workspace(D, max_q, group, max_len, batch, kv_heads);
-    const int64_t tiles = in_tiles(D, max_q, group) ? prefill_workspace(tokens, batch, group, kv_heads, D, max_len) : 0;
+    const int64_t tiles = in_tiles(max_q, group) ? prefill_workspace(tokens, batch, group, kv_heads, D, max_len) : 0;
     return streamed > tiles ? streamed : tiles;  // (used one after the other)
 }
 
@@ -832,7 +854,7 @@ extern "C" int xg_kv4_attention(const void* q, const void* cache, int64_t pages,
         return fail(XG_ERR_INVALID_ARG, "xg_kv4_attention: needs %lld bytes of 16-byte aligned workspace", (long long)need);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     // Sequences with many columns go to the tensor-memory kernel, where there may be any; the others to the streaming one.
-    const bool tiles = batch > 0 && in_tiles(D, max_q, p.group);
+    const bool tiles = batch > 0 && in_tiles(max_q, p.group);
     const int most = tiles ? kMostStreamed : 0x7fffffff;
     const int rc = dtype == XG_BF16 ? attend_split<__nv_bfloat16>(p, D, max_q, most, workspace, st) : attend_split<__half>(p, D, max_q, most, workspace, st);
     return rc != XG_OK || !tiles ? rc : attend_prefill(p, D, dtype, most, workspace, st);

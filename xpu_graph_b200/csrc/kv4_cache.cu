@@ -1,7 +1,7 @@
 // Keys and values in 4 bits: quantising new tokens into cache pages, reading tokens back, copying pages. All three move bytes and
 // are bound by HBM (the layout: kv4_tile.cuh).
 //
-// Quantising, per token, head and group of 64 channels: least = fp16(min x), scale = fp16((max x - least) / 15),
+// Quantising, per token, head and group of 64 channels: least = fp16(min x), scale = fp16((max x - least) * fp32(1/15)),
 // code = rint((x - least) / scale) in 0..15, every step in fp32 with IEEE rounding. The fp16 roundings of the pair come first,
 // so the codes are the nearest ones for the pair that is stored.
 #include "kv4_tile.cuh"
@@ -87,7 +87,7 @@ __device__ __forceinline__ void quantise(const Raw8<T> (&x)[2], uint32_t (&word)
     if (lo == lo) lo = fminf(fmaxf(lo, -kLargest), kLargest);
     const __half least = __float2half_rn(lo);
     const float least_f = __half2float(least);
-    const __half scale = __float2half_rn(__fdiv_rn(hi - least_f, 15.0f));
+    const __half scale = __float2half_rn(__fmul_rn(hi - least_f, 1.0f / 15.0f));
     const float scale_f = __half2float(scale);
     pair = (uint32_t)__half_as_ushort(scale) | ((uint32_t)__half_as_ushort(least) << 16);
     word[0] = word[1] = 0;

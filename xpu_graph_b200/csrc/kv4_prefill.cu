@@ -1,7 +1,7 @@
 // Attention of many new tokens over the 4-bit cache: flash attention on tcgen05 with keys and values unpacked on the way in.
 //
 // A CTA owns 256 rows of one kv head - rows are the (new token, head of the group) pairs in token order, so that all heads of a group
-// share the unpacked keys - as two 128-row tiles. Per block of 64 keys: four warps unpack K and V, one 16-key tile each, from a ring of
+// share the unpacked keys - as two 128-row tiles (one at head dim 256). Per block of 64 keys: warps unpack K and V from a ring of
 // bulk copies into fp16 operand tiles (128-byte swizzle, the layout a tensor map would leave); one thread issues S = Q K^T for both
 // tiles into double-buffered tensor memory, then O += P V with P read from tensor memory; eight warps (a row per thread) turn
 // scores into probabilities in place, as flash_tc_kernel (sdpa.cu) does, with the maximum lagging by up to 2^8.
@@ -23,17 +23,24 @@ using namespace kv4;
 
 constexpr int PM = 128;  // rows per tile
 constexpr int PN = 64;   // keys per block
-constexpr int kUnpackWarps = 4, kRing = 4;
-constexpr int kPrefillThreads = (kUnpackWarps + 1 + 8) * 32;
+constexpr int kBlockTiles = PN / kTileTokens;
+constexpr int kPrefillThreads = 13 * 32;  // unpacking, one warp for the products, softmax
 constexpr float kLag = 8.0f;  // log2 units
 
 template <int D>
 struct PreCfg {
+    // Two tiles of rows share the unpacked keys, so that unpacking is half as much per product; at head dim 256 neither tensor memory
+    // (two outputs would fill it) nor shared memory has room for them, nor for a second buffer of V. Twice the warps unpack then.
+    static constexpr int TILES = D == 256 ? 1 : 2, VBUF = TILES, UNPACK = TILES == 2 ? 4 : 8, RING_STAGES = TILES == 2 ? 4 : 2;
+    static constexpr int ROWS = TILES * PM;
+    static constexpr int HALVES = UNPACK / kBlockTiles, TOKENS = kTileTokens / HALVES;  // a warp's tokens of a tile
     static constexpr int Q_BYTES = PM * D * 2;
     static constexpr int KV_BYTES = PN * D * 2;
-    static constexpr int TILE = tile_bytes(D);
-    static constexpr int RING = kUnpackWarps * kRing * TILE;
-    static constexpr int SMEM = 2 * Q_BYTES + 4 * KV_BYTES + RING + 512;
+    static constexpr int TILE = tile_bytes(D), STAGE = TILE / HALVES;  // of the ring
+    static constexpr int RING = UNPACK * RING_STAGES * STAGE;
+    static constexpr int SMEM = TILES * Q_BYTES + (2 + VBUF) * KV_BYTES + RING + 768;
+    static constexpr uint32_t O_COL = TILES * 2 * PN;  // tensor memory: two score buffers per tile, then the outputs
+    static_assert(O_COL + TILES * D <= 512 && SMEM <= 232448, "fits an SM");
 };
 
 struct Unit {
@@ -69,10 +76,11 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
     using Cfg = PreCfg<D>;
     constexpr int W = D / 32, GR = D / 64;
     extern __shared__ __align__(1024) uint8_t smem[];
-    uint8_t* q_s = smem;                          // [2][Q_BYTES]; at the end the output rows on their way out
-    uint8_t* k_s = q_s + 2 * Cfg::Q_BYTES;        // [2][KV_BYTES]
-    uint8_t* v_s = k_s + 2 * Cfg::KV_BYTES;       // [2][KV_BYTES]
-    uint8_t* ring = v_s + 2 * Cfg::KV_BYTES;
+    constexpr int TILES = Cfg::TILES, UNPACK = Cfg::UNPACK, STAGES = Cfg::RING_STAGES;
+    uint8_t* q_s = smem;                                  // [TILES][Q_BYTES]; at the end the output rows on their way out
+    uint8_t* k_s = q_s + TILES * Cfg::Q_BYTES;            // [2][KV_BYTES]
+    uint8_t* v_s = k_s + 2 * Cfg::KV_BYTES;               // [VBUF][KV_BYTES]
+    uint8_t* ring = v_s + Cfg::VBUF * Cfg::KV_BYTES;
     uint64_t* bars = reinterpret_cast<uint64_t*>(ring + Cfg::RING);
     uint64_t* q_full = bars;          // [tile]
     uint64_t* k_full = bars + 2;      // [buffer]
@@ -85,12 +93,12 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
     uint64_t* o_full = bars + 20;     // [tile]
     uint64_t* drain_bar = bars + 22;
     uint64_t* ring_full = bars + 23;  // [warp][stage]
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 23 + kUnpackWarps * kRing);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 23 + UNPACK * STAGES);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    volatile int* holes = abort_flag + 1;                    // [4][warp]: a block's tiles that are not in the cache
-    volatile int* ring_hole = holes + 4 * kUnpackWarps;      // [warp][stage]
-    Unit* unit = reinterpret_cast<Unit*>(const_cast<int*>(ring_hole + kUnpackWarps * kRing));
-    static_assert(23 * 8 + kUnpackWarps * kRing * 8 + 8 + (4 * kUnpackWarps + kUnpackWarps * kRing) * 4 + sizeof(Unit) <= 512, "barriers");
+    volatile int* holes = abort_flag + 1;              // [4][warp]: a block's tiles that are not in the cache
+    volatile int* ring_hole = holes + 4 * UNPACK;      // [warp][stage]
+    Unit* unit = reinterpret_cast<Unit*>(const_cast<int*>(ring_hole + UNPACK * STAGES));
+    static_assert(23 * 8 + UNPACK * STAGES * 8 + 8 + (4 * UNPACK + UNPACK * STAGES) * 4 + sizeof(Unit) <= 768, "barriers");
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if ((ptx::smem_u32(smem) & 1023u) != 0) {  // uniform over the CTA: the swizzled tiles need this alignment
@@ -101,9 +109,9 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             ptx::mbar_init(&q_full[i], PM);
-            ptx::mbar_init(&k_full[i], kUnpackWarps);
+            ptx::mbar_init(&k_full[i], UNPACK);
             ptx::mbar_init(&k_empty[i], 1);
-            ptx::mbar_init(&v_full[i], kUnpackWarps);
+            ptx::mbar_init(&v_full[i], UNPACK);
             ptx::mbar_init(&v_empty[i], 1);
             ptx::mbar_init(&pv_full[i], 1);
             ptx::mbar_init(&o_full[i], 1);
@@ -113,12 +121,12 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
             ptx::mbar_init(&p_full[i], PM);
         }
         ptx::mbar_init(drain_bar, 1);
-        for (int i = 0; i < kUnpackWarps * kRing; ++i) ptx::mbar_init(&ring_full[i], 1);
+        for (int i = 0; i < UNPACK * STAGES; ++i) ptx::mbar_init(&ring_full[i], 1);
         *abort_flag = 0;
         ptx::fence_mbar_init();
         ptx::fence_proxy_async();
     }
-    if (warp == kUnpackWarps) ptx::tmem_alloc(tmem_slot, 512);
+    if (warp == UNPACK) ptx::tmem_alloc(tmem_slot, 512);
     pdl_sync();
     if (warp == 0) {  // which rows are this CTA's: the sequences' units one after the other, the last rows (most keys) first
         int base = 0;
@@ -129,7 +137,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
             int w = 0;
             if (b < p.batch) {
                 s = sequence(p, b);
-                if (s.count * p.group > beyond) w = (s.count * p.group + 2 * PM - 1) / (2 * PM) * p.cache.heads;
+                if (s.count * p.group > beyond) w = (s.count * p.group + Cfg::ROWS - 1) / Cfg::ROWS * p.cache.heads;
             }
             int inc = w;
 #pragma unroll
@@ -157,8 +165,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
     const int rows = u.count * p.group;
     // key blocks of a tile: up to what its last row sees
     auto blocks_of = [&](int i) {
-        const int lo = u.rt * 2 * PM + i * PM;
-        if (!u.on || lo >= rows) return 0;
+        const int lo = u.rt * Cfg::ROWS + i * PM;
+        if (!u.on || i >= TILES || lo >= rows) return 0;
         const int seen = u.len - u.count + (min(rows, lo + PM) - 1) / p.group + 1;
         return seen > 0 ? (seen + PN - 1) / PN : 0;
     };
@@ -168,53 +176,66 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
     const int nblk0 = min(nblk, max(0, blocks_of(0) - j0)), nblk1 = min(nblk, max(0, blocks_of(1) - j0));
     if (parts.splits > 1 && split == 0 && threadIdx.x == 0) parts.unit[blockIdx.x / parts.splits] = u;
 
-    if (warp < kUnpackWarps) {
+    if (warp < UNPACK) {
         // ------------------------------ unpacking ---------------------------------
-        uint8_t* my_ring = ring + warp * (kRing * Cfg::TILE);
-        uint64_t* my_full = ring_full + warp * kRing;
-        volatile int* my_hole = ring_hole + warp * kRing;
+        const int mine = warp / Cfg::HALVES, h = warp % Cfg::HALVES;  // tile of the block, which of its tokens: TOKENS h and on
+        uint8_t* my_ring = ring + warp * (STAGES * Cfg::STAGE);   // a stage: codes of keys, of values, pairs of keys, of values
+        uint64_t* my_full = ring_full + warp * STAGES;
+        volatile int* my_hole = ring_hole + warp * STAGES;
         int64_t addr = 0;
         auto issue = [&](int j) {  // this warp's tile of block j
             if (j >= nblk) return;
             if ((j & 31) == 0) {
-                const int tile = (j0 + j + lane) * kUnpackWarps + warp;
+                const int tile = (j0 + j + lane) * kBlockTiles + mine;
                 addr = tile * kTileTokens < u.len ? tile_of_token(p, u.b, u.kvh, tile, Cfg::TILE) : 0;
             }
             const int64_t from = __shfl_sync(0xffffffffu, addr, j & 31);
-            const int stage = j % kRing;
+            const int stage = j % STAGES;
             if (lane == 0) {
                 my_hole[stage] = from == 0;
                 if (from != 0) {
-                    ptx::mbar_arrive_expect_tx(&my_full[stage], Cfg::TILE);
-                    ptx::bulk_load(my_ring + stage * Cfg::TILE, reinterpret_cast<const void*>(from), Cfg::TILE, &my_full[stage]);
+                    ptx::mbar_arrive_expect_tx(&my_full[stage], Cfg::STAGE);
+                    uint8_t* dst = my_ring + stage * Cfg::STAGE;
+                    const uint8_t* src = reinterpret_cast<const uint8_t*>(from);
+                    if (Cfg::HALVES == 1) {
+                        ptx::bulk_load(dst, src, Cfg::TILE, &my_full[stage]);
+                    } else {  // (a half of a tile's tokens is a half of each of its four parts)
+                        constexpr int C = 8 * D / Cfg::HALVES, P = D / Cfg::HALVES;
+                        ptx::bulk_load(dst, src + h * C, C, &my_full[stage]);
+                        ptx::bulk_load(dst + C, src + 8 * D + h * C, C, &my_full[stage]);
+                        ptx::bulk_load(dst + 2 * C, src + 16 * D + h * P, P, &my_full[stage]);
+                        ptx::bulk_load(dst + 2 * C + P, src + 17 * D + h * P, P, &my_full[stage]);
+                    }
                 } else {
                     ptx::mbar_arrive(&my_full[stage]);
                 }
             }
         };
-        for (int j = 0; j < kRing; ++j) issue(j);
+        for (int j = 0; j < STAGES; ++j) issue(j);
         const __half2 zero = __half2half2(__ushort_as_half(0));
         bool ok = true;
         // keys: a lane takes chunk t of rows r and r + 8; the bits are dealt so that neither its reads nor its swizzled writes collide
         const int kr = (lane & 1) | ((lane >> 3) & 1) << 1 | ((lane >> 1) & 1) << 2, kt = ((lane >> 4) & 1) | ((lane >> 2) & 1) << 1;
         for (int j = 0; j < nblk; ++j) {
-            const int stage = j % kRing, buf = j & 1;
+            const int stage = j % STAGES, buf = j & 1;
             const uint32_t ph = (uint32_t)(j >> 1) & 1u;
-            if (!__all_sync(0xffffffffu, ptx::mbar_wait_bounded(&my_full[stage], (uint32_t)(j / kRing) & 1u, abort_flag))) { ok = false; break; }
-            const uint8_t* tile = my_ring + stage * Cfg::TILE;
+            if (!__all_sync(0xffffffffu, ptx::mbar_wait_bounded(&my_full[stage], (uint32_t)(j / STAGES) & 1u, abort_flag))) { ok = false; break; }
+            constexpr int C = 8 * D / Cfg::HALVES, P = D / Cfg::HALVES;
+            const uint8_t* codes = my_ring + stage * Cfg::STAGE;
+            const uint8_t* pair_s = codes + 2 * C;  // a token's pairs D / 16 bytes apart
             const int hole = my_hole[stage];
-            const int there = hole ? 0 : u.len - ((j0 + j) * kUnpackWarps + warp) * kTileTokens;  // tokens of the tile that exist
+            const int there = hole ? 0 : u.len - ((j0 + j) * kBlockTiles + mine) * kTileTokens - h * Cfg::TOKENS;  // of this warp's tokens
             if (!__all_sync(0xffffffffu, ptx::mbar_wait_bounded(&k_empty[buf], ph ^ 1u, abort_flag))) { ok = false; break; }
-            if (lane == 0) holes[(j & 3) * kUnpackWarps + warp] = hole;
+            if (lane == 0) holes[(j & 3) * UNPACK + warp] = hole;
             {
-                const uint32_t base = ptx::smem_u32(k_s + buf * Cfg::KV_BYTES) + (uint32_t)(warp * kTileTokens * 128);
+                const uint32_t base = ptx::smem_u32(k_s + buf * Cfg::KV_BYTES) + (uint32_t)(warp * Cfg::TOKENS * 128);
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
+                for (int half = 0; half < Cfg::TOKENS / 8; ++half) {
                     const int r = kr + 8 * half;
                     uint32_t words[W];
                     __half2 pairs[GR];
-                    load_words<W>(tile + r * (D / 2) + kt * (D / 8), words);
-                    load_pairs<GR>(tile + pair_at(D, 0, r, 0), pairs);
+                    load_words<W>(codes + r * (D / 2) + kt * (D / 8), words);
+                    load_pairs<GR>(pair_s + r * (D / 16), pairs);
 #pragma unroll
                     for (int gr = 0; gr < GR; ++gr) {
                         const __half2 pair = r < there ? pairs[gr] : zero, scale = __low2half2(pair), least = __high2half2(pair);
@@ -227,17 +248,18 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
             ptx::fence_proxy_async();
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(&k_full[buf]);
-            if (!__all_sync(0xffffffffu, ptx::mbar_wait_bounded(&v_empty[buf], ph ^ 1u, abort_flag))) { ok = false; break; }
+            const int vbuf = Cfg::VBUF == 2 ? buf : 0;
+            if (!__all_sync(0xffffffffu, ptx::mbar_wait_bounded(&v_empty[vbuf], (Cfg::VBUF == 2 ? ph : (uint32_t)j & 1u) ^ 1u, abort_flag))) { ok = false; break; }
             {
-                const uint32_t base = ptx::smem_u32(v_s + buf * Cfg::KV_BYTES) + (uint32_t)(warp * kTileTokens * 128);
+                const uint32_t base = ptx::smem_u32(v_s + vbuf * Cfg::KV_BYTES) + (uint32_t)(warp * Cfg::TOKENS * 128);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < Cfg::TOKENS / 4; ++i) {  // (rows of value codes: 8 tokens' are a half of the tile's as well)
                     const int at = i * 4 + (lane >> 3), t = at & 3, c = at >> 2, r = 2 * t + (c & 1) + 8 * (c >> 1);
                     const int place = lane & 7, chunk = place ^ (2 * t);
                     uint32_t words[GR];
                     __half2 pairs[GR];
-                    load_words<GR>(tile + 8 * D + at * (D / 2) + place * (D / 16), words);
-                    load_pairs<GR>(tile + pair_at(D, 1, r, 0), pairs);
+                    load_words<GR>(codes + C + at * (D / 2) + place * (D / 16), words);
+                    load_pairs<GR>(pair_s + P + r * (D / 16), pairs);
 #pragma unroll
                     for (int w = 0; w < GR; ++w) {
                         const __half2 pair = r < there ? pairs[w] : zero;
@@ -248,8 +270,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
             }
             ptx::fence_proxy_async();
             __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(&v_full[buf]);
-            issue(j + kRing);
+            if (lane == 0) ptx::mbar_arrive(&v_full[vbuf]);
+            issue(j + STAGES);
         }
         if (!ok) {
             if (lane == 0) atomicOr(&g_kv4_prefill_status[0], 1u);
@@ -257,7 +279,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
             while (ptx::globaltimer_ns() - t0 < 20000ull) {
             }
         }
-    } else if (warp == kUnpackWarps) {
+    } else if (warp == UNPACK) {
         // ------------------------------ products ----------------------------------
         if (ptx::elect_one()) {
             constexpr uint32_t idesc_s = ptx::make_idesc_f16(0, PM, PN, 0);
@@ -270,7 +292,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
                 if (!ptx::mbar_wait_bounded(&k_full[buf], (uint32_t)(j >> 1) & 1u, abort_flag)) return false;
                 ptx::tc_fence_after();
                 const uint32_t k_addr = ptx::smem_u32(k_s + buf * Cfg::KV_BYTES);
-                for (int i = 0; i < 2; ++i) {
+                for (int i = 0; i < TILES; ++i) {
                     if (j >= (i ? nblk1 : nblk0)) continue;
                     if (j == 0 && !ptx::mbar_wait_bounded(&q_full[i], 0, abort_flag)) return false;
                     if (j == 0) ptx::tc_fence_after();
@@ -290,21 +312,22 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
                 if (j + 1 < nblk && !issue_qk(j + 1)) { ok = false; break; }
                 const int buf = j & 1;
                 const uint32_t ph = (uint32_t)(j >> 1) & 1u;
-                if (!ptx::mbar_wait_bounded(&v_full[buf], ph, abort_flag)) { ok = false; break; }
-                const uint32_t v_addr = ptx::smem_u32(v_s + buf * Cfg::KV_BYTES);
-                for (int i = 0; i < 2 && ok; ++i) {
+                const int vbuf = Cfg::VBUF == 2 ? buf : 0;
+                if (!ptx::mbar_wait_bounded(&v_full[vbuf], Cfg::VBUF == 2 ? ph : (uint32_t)j & 1u, abort_flag)) { ok = false; break; }
+                const uint32_t v_addr = ptx::smem_u32(v_s + vbuf * Cfg::KV_BYTES);
+                for (int i = 0; i < TILES && ok; ++i) {
                     const int n = i ? nblk1 : nblk0;
                     if (j >= n) continue;
                     if (!ptx::mbar_wait_bounded(&p_full[2 * i + buf], ph, abort_flag)) { ok = false; break; }
                     ptx::tc_fence_after();
 #pragma unroll
                     for (int kk = 0; kk < PN / 16; ++kk)  // P: 16 keys = 8 columns of packed pairs per step, over its scores
-                        ptx::mma_f16_ts(tmem_base + 256u + (uint32_t)(i * 128), tmem_base + (uint32_t)((2 * i + buf) * PN + kk * 8),
+                        ptx::mma_f16_ts(tmem_base + Cfg::O_COL + (uint32_t)(i * D), tmem_base + (uint32_t)((2 * i + buf) * PN + kk * 8),
                                         ptx::make_mnmajor_sw128_desc(v_addr + (uint32_t)(kk * 16 * 128), PN * 128), idesc_o, (j | kk) != 0 ? 1u : 0u);
                     ptx::tc_commit(&pv_full[i]);
                     if (j + 1 == n) ptx::tc_commit(&o_full[i]);
                 }
-                if (ok) ptx::tc_commit(&v_empty[buf]);
+                if (ok) ptx::tc_commit(&v_empty[vbuf]);
             }
             if (!ok) {
                 atomicOr(&g_kv4_prefill_status[0], 2u);
@@ -317,10 +340,10 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
         }
     } else {
         // ------------------------------ softmax / output rows ---------------------
-        const int i = (warp - kUnpackWarps - 1) >> 2, quad = warp & 3;
+        const int i = (warp - UNPACK - 1) >> 2, quad = warp & 3;
         const int r_in_tile = quad * 32 + lane;
         const int n = i ? nblk1 : nblk0;
-        const int lo = u.rt * 2 * PM + i * PM;
+        const int lo = u.rt * Cfg::ROWS + i * PM;
         const int row = lo + r_in_tile;
         const bool there = u.on && row < rows;
         const int token = there ? row / p.group : 0;
@@ -331,12 +354,11 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
             // this row of q, a power of two taken out, into the operand tile
             const T* q = reinterpret_cast<const T*>(p.q) + (int64_t)(u.first + token) * p.q_st + (int64_t)head * p.q_sh;
             const bool vec = (reinterpret_cast<uintptr_t>(p.q) & 15) == 0 && p.q_st % 8 == 0 && p.q_sh % 8 == 0;
-            uint4 raw[D / 8];
             float top = 0.f;
-#pragma unroll
+#pragma unroll 4
             for (int c = 0; c < D / 8; ++c) {
-                raw[c] = there ? load_q8(q + 8 * c, vec) : make_uint4(0, 0, 0, 0);
-                const T* e = reinterpret_cast<const T*>(&raw[c]);
+                const uint4 raw = there ? load_q8(q + 8 * c, vec) : make_uint4(0, 0, 0, 0);
+                const T* e = reinterpret_cast<const T*>(&raw);
 #pragma unroll
                 for (int x = 0; x < 8; ++x) top = fmaxf(top, fabsf(Cvt<T>::to_f(e[x])));
             }
@@ -347,9 +369,10 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
             if (p.scale < 0.f) down = -down;
             mul = fmaxf((p.scale == 0.f ? 1.f : fabsf(p.scale)) * kLog2e * __uint_as_float((uint32_t)(127 + e) << 23), 1e-37f);
             const uint32_t base = ptx::smem_u32(q_s + i * Cfg::Q_BYTES) + (uint32_t)(r_in_tile * 128);
-#pragma unroll
-            for (int c = 0; c < D / 8; ++c) {
-                const T* e8 = reinterpret_cast<const T*>(&raw[c]);
+#pragma unroll 4
+            for (int c = 0; c < D / 8; ++c) {  // (the row once more, from the cache)
+                const uint4 raw = there ? load_q8(q + 8 * c, vec) : make_uint4(0, 0, 0, 0);
+                const T* e8 = reinterpret_cast<const T*>(&raw);
                 uint32_t w[4];
 #pragma unroll
                 for (int x = 0; x < 4; ++x) w[x] = ptx::pack2<__half>(Cvt<T>::to_f(e8[x]) * down, Cvt<T>::to_f(e8[x + 4]) * down);  // (unpack8's order)
@@ -359,7 +382,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
             ptx::mbar_arrive(&q_full[i]);
         }
         const uint32_t lane_field = (uint32_t)(quad * 32) << 16;
-        const uint32_t o_taddr = tmem_base + lane_field + 256u + (uint32_t)(i * 128);
+        const uint32_t o_taddr = tmem_base + lane_field + Cfg::O_COL + (uint32_t)(i * D);
         bool ok = true;
         float m_run = -INFINITY, l_run = 0.f;
         for (int j = 0; j < n; ++j) {
@@ -370,7 +393,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
             const int visible = limit - (j0 + j) * PN;  // columns of this block that the row sees
             int hole = 0;
 #pragma unroll
-            for (int w = 0; w < kUnpackWarps; ++w) hole |= (holes[(j & 3) * kUnpackWarps + w] != 0) << w;
+            for (int w = 0; w < kBlockTiles; ++w) hole |= (holes[(j & 3) * UNPACK + w * Cfg::HALVES] != 0) << w;
             if (__all_sync(0xffffffffu, visible <= 0) || hole == 15) {  // probabilities of zero; maximum and sum stay
                 uint32_t zero[32];
 #pragma unroll
@@ -462,11 +485,11 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
         if (ok && n > 0) ok = __all_sync(0xffffffffu, ptx::mbar_wait_bounded(&o_full[i], 0, abort_flag)) != 0;
         if (ok && parts.splits > 1 && there) {
             ptx::tc_fence_after();
-            const int64_t at = (int64_t)blockIdx.x * (2 * PM) + i * PM + r_in_tile;
+            const int64_t at = (int64_t)blockIdx.x * Cfg::ROWS + i * PM + r_in_tile;
             parts.ml[at] = make_float2(m_run, l_run);
         }
         if (ok && parts.splits > 1 && u.on && lo + quad * 32 < rows) {
-            const int64_t at = (int64_t)blockIdx.x * (2 * PM) + i * PM + r_in_tile;
+            const int64_t at = (int64_t)blockIdx.x * Cfg::ROWS + i * PM + r_in_tile;
 #pragma unroll 1
             for (int c = 0; c < D / 32 && n > 0; ++c) {
                 uint32_t o[32];
@@ -525,7 +548,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
 
     ptx::tc_fence_before();
     __syncthreads();
-    if (warp == kUnpackWarps) {
+    if (warp == UNPACK) {
         ptx::tc_fence_after();
         ptx::tmem_dealloc(tmem_base, 512);
     }
@@ -537,9 +560,10 @@ __global__ void __launch_bounds__(256) kv4_prefill_combine_kernel(const AttendPa
     pdl_sync();
     const Unit u = parts.unit[blockIdx.x];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int in_unit = blockIdx.y * 8 + warp, row = u.rt * 2 * PM + in_unit;
+    constexpr int ROWS = PreCfg<D>::ROWS;
+    const int in_unit = blockIdx.y * 8 + warp, row = u.rt * ROWS + in_unit;
     if (!u.on || row >= u.count * p.group) return;
-    auto at = [&](int i) { return ((int64_t)blockIdx.x * parts.splits + i) * (2 * PM) + in_unit; };
+    auto at = [&](int i) { return ((int64_t)blockIdx.x * parts.splits + i) * ROWS + in_unit; };
     float m = -INFINITY;
     for (int i = lane; i < parts.splits; i += 32) m = fmaxf(m, parts.ml[at(i)].x);
     m = warp_max(m);
@@ -567,7 +591,7 @@ __global__ void __launch_bounds__(256) kv4_prefill_combine_kernel(const AttendPa
 }
 
 // The most units there can be, and over how many CTAs each one's keys are shared out: as many as fill the chip once, 512 keys or more each.
-int64_t most_units(int64_t tokens, int64_t batch, int64_t group, int64_t heads) { return (tokens * group + batch * (2 * PM - 1)) / (2 * PM) * heads; }
+int64_t most_units(int64_t tokens, int64_t batch, int64_t group, int64_t heads, int64_t rows) { return (tokens * group + batch * (rows - 1)) / rows * heads; }
 int key_splits(int64_t units, int64_t max_len) {
     int64_t n = num_sms() / (units > 0 ? units : 1);
     if (n > max_len / 512) n = max_len / 512;
@@ -580,12 +604,12 @@ int launch_prefill(const AttendParams& p, int beyond, void* workspace, cudaStrea
     static std::atomic<uint64_t> reserved;
     if (!reserve_smem(kv4_prefill_kernel<T, D>, Cfg::SMEM, reserved)) return fail(XG_ERR_LAUNCH, "xg_kv4_attention: cannot reserve shared memory");
     // at least as many CTAs as there are units; those behind the last one return at once
-    const int64_t units = most_units(p.tokens, p.batch, p.group, p.cache.heads);
+    const int64_t units = most_units(p.tokens, p.batch, p.group, p.cache.heads, Cfg::ROWS);
     Parts parts = {};
     parts.splits = key_splits(units, (int64_t)p.table_pages * p.cache.tiles * kTileTokens);
     if (units * parts.splits > 0x7fffffffLL) return fail(XG_ERR_TOO_LARGE, "xg_kv4_attention: too many rows");
     if (parts.splits > 1) {
-        const int64_t rows = units * parts.splits * 2 * PM;
+        const int64_t rows = units * parts.splits * Cfg::ROWS;
         parts.rows = static_cast<float*>(workspace);
         parts.ml = reinterpret_cast<float2*>(parts.rows + rows * D);
         parts.unit = reinterpret_cast<Unit*>(parts.ml + rows);
@@ -593,21 +617,25 @@ int launch_prefill(const AttendParams& p, int beyond, void* workspace, cudaStrea
     launch_with({.early = false}, kv4_prefill_kernel<T, D>, (unsigned)(units * parts.splits), kPrefillThreads, Cfg::SMEM, st, p, beyond, parts);
     if (const int rc = check_launch("xg_kv4_attention")) return rc;
     if (parts.splits == 1) return XG_OK;
-    launch(kv4_prefill_combine_kernel<T, D>, dim3((unsigned)units, 2 * PM / 8), 256, 0, st, p, parts);
+    launch(kv4_prefill_combine_kernel<T, D>, dim3((unsigned)units, Cfg::ROWS / 8), 256, 0, st, p, parts);
     return check_launch("xg_kv4_attention");
 }
 
 }  // namespace
 
 int64_t prefill_workspace(int64_t tokens, int64_t batch, int64_t group, int64_t heads, int64_t D, int64_t max_len) {
-    const int64_t units = most_units(tokens, batch, group, heads);
+    const int64_t rows = D == 256 ? PreCfg<256>::ROWS : PreCfg<128>::ROWS, units = most_units(tokens, batch, group, heads, rows);
     const int splits = key_splits(units, max_len);
-    return splits == 1 ? 0 : units * splits * 2 * PM * (D + 2) * 4 + units * (int64_t)sizeof(Unit);
+    return splits == 1 ? 0 : units * splits * rows * (D + 2) * 4 + units * (int64_t)sizeof(Unit);
 }
 
 int attend_prefill(const AttendParams& p, int64_t D, int dtype, int beyond, void* workspace, cudaStream_t st) {
-    if (dtype == XG_BF16) return D == 64 ? launch_prefill<__nv_bfloat16, 64>(p, beyond, workspace, st) : launch_prefill<__nv_bfloat16, 128>(p, beyond, workspace, st);
-    return D == 64 ? launch_prefill<__half, 64>(p, beyond, workspace, st) : launch_prefill<__half, 128>(p, beyond, workspace, st);
+    const bool bf16 = dtype == XG_BF16;
+    switch (D) {
+        case 64: return bf16 ? launch_prefill<__nv_bfloat16, 64>(p, beyond, workspace, st) : launch_prefill<__half, 64>(p, beyond, workspace, st);
+        case 128: return bf16 ? launch_prefill<__nv_bfloat16, 128>(p, beyond, workspace, st) : launch_prefill<__half, 128>(p, beyond, workspace, st);
+        default: return bf16 ? launch_prefill<__nv_bfloat16, 256>(p, beyond, workspace, st) : launch_prefill<__half, 256>(p, beyond, workspace, st);
+    }
 }
 
 int read_kv4_prefill_status(unsigned int* host_out, int reset) {
