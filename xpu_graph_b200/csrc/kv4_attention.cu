@@ -678,42 +678,63 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
 }
 
 // The parts of the unit that starts in range blockIdx.x and goes on in others: out = sum 2^(m_i - m) O_i / sum 2^(m_i - m) l_i. A CTA per
-// range (most have nothing to do and leave), SPLIT warps per column that take the parts in turn: a sequence may fill every range.
+// range (some have nothing to do and leave), SPLIT warps per column that take the parts in turn: a sequence may fill every range, but
+// mostly there are two or three. 512 threads, so that all CTAs fit the chip at once (1024: 9 us behind 64 sequences, this 6).
+constexpr int kCombineThreads = 512;
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(1024) kv4_combine_kernel(const SplitParams sp, int ranges) {
+__global__ void __launch_bounds__(kCombineThreads, 3) kv4_combine_kernel(const SplitParams sp, int ranges) {
     using Cfg = SplitCfg<D, NT>;
-    constexpr int SPLIT = 32 / Cfg::COLS, C = D / 32;
+    constexpr int WARPS = kCombineThreads / 32, SPLIT = WARPS / Cfg::COLS, C = D / 32;
     pdl_sync();
-    const PartDesc d = reinterpret_cast<const PartDesc*>(sp.parts + (int64_t)2 * ranges * Cfg::part_floats())[blockIdx.x];
-    if (d.parts == 0) return;
-    __shared__ __align__(16) float o_s[32][D];
-    __shared__ float2 ml_s[32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = warp / SPLIT;
     const float2* ml = reinterpret_cast<const float2*>(sp.parts + (int64_t)2 * ranges * Cfg::COLS * D);
     auto slot = [&](int i) { return (2 * ((int64_t)blockIdx.x + i) + (i == 0 ? 1 : 0)) * Cfg::COLS + col; };
-    const bool on = d.ct * Cfg::COLS + col < d.count * sp.a.group;
-    float m = -INFINITY, l = 0.f, o[C];
+    // (what the first parts would be is fetched along with the word that says how many there are)
+    const bool in = (int)blockIdx.x + lane < ranges;
+    const float2 mine = in ? ml[slot(lane)] : make_float2(-INFINITY, 0.f);
+    const PartDesc d = reinterpret_cast<const PartDesc*>(sp.parts + (int64_t)2 * ranges * Cfg::part_floats())[blockIdx.x];
+    if (d.parts == 0) return;
+    __shared__ __align__(16) float o_s[WARPS][D];
+    __shared__ float l_s[WARPS];
+    float m = lane < d.parts ? mine.x : -INFINITY, l = 0.f, o[C];
 #pragma unroll
     for (int c = 0; c < C; ++c) o[c] = 0.f;
-    if (on) {
-        for (int i = lane; i < d.parts; i += 32) m = fmaxf(m, ml[slot(i)].x);
+    if (d.ct * Cfg::COLS + col < d.count * sp.a.group) {
+        for (int i = 32 + lane; i < d.parts; i += 32) m = fmaxf(m, ml[slot(i)].x);
         m = warp_max(m);
         const float use = m == -INFINITY ? 0.f : m;
-#pragma unroll 4
-        for (int i = warp % SPLIT; i < d.parts; i += SPLIT) {
-            const float2 part = ml[slot(i)];
-            const float* src = sp.parts + slot(i) * D + lane;
-            const float f = ptx::ex2_approx(part.x - use);
-            l = fmaf(part.y, f, l);
+        constexpr int AHEAD = D == 256 ? 2 : 4;  // parts in flight
+#pragma unroll 1
+        for (int i0 = warp % SPLIT; i0 < d.parts; i0 += AHEAD * SPLIT) {
+            float v[AHEAD][C];
+            float2 part[AHEAD];
 #pragma unroll
-            for (int c = 0; c < C; ++c) o[c] = fmaf(src[c * 32], f, o[c]);
+            for (int j = 0; j < AHEAD; ++j) {
+                const int i = i0 + j * SPLIT;
+                const float x = __shfl_sync(0xffffffffu, mine.x, i & 31), y = __shfl_sync(0xffffffffu, mine.y, i & 31);
+                part[j] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+                for (int c = 0; c < C; ++c) v[j][c] = 0.f;
+                if (i < d.parts) {
+                    part[j] = i < 32 ? make_float2(x, y) : ml[slot(i)];
+#pragma unroll
+                    for (int c = 0; c < C; ++c) v[j][c] = sp.parts[slot(i) * D + c * 32 + lane];
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                const float f = ptx::ex2_approx(part[j].x - use);
+                l = fmaf(part[j].y, f, l);
+#pragma unroll
+                for (int c = 0; c < C; ++c) o[c] = fmaf(v[j][c], f, o[c]);
+            }
         }
     }
 #pragma unroll
     for (int c = 0; c < C; ++c) o_s[warp][c * 32 + lane] = o[c];
-    if (lane == 0) ml_s[warp].x = l;
+    if (lane == 0) l_s[warp] = l;
     __syncthreads();
-    for (int i = threadIdx.x; i < Cfg::COLS * (D / 8); i += 1024) {
+    for (int i = threadIdx.x; i < Cfg::COLS * (D / 8); i += kCombineThreads) {
         const int at = i / (D / 8), ch = (i - at * (D / 8)) * 8, pair = d.ct * Cfg::COLS + at;
         if (pair >= d.count * sp.a.group) break;
         float sum = 0.f, y[8];
@@ -721,7 +742,7 @@ __global__ void __launch_bounds__(1024) kv4_combine_kernel(const SplitParams sp,
         for (int e = 0; e < 8; ++e) y[e] = 0.f;
 #pragma unroll
         for (int w = at * SPLIT; w < (at + 1) * SPLIT; ++w) {
-            sum += ml_s[w].x;
+            sum += l_s[w];
 #pragma unroll
             for (int e = 0; e < 8; ++e) y[e] += o_s[w][ch + e];
         }
@@ -742,7 +763,7 @@ int launch_split(SplitParams sp, cudaStream_t st) {
     launch_with({.early = false}, kv4_split_kernel<T, D, NT>, (unsigned)grid, kWarps * 32, (size_t)bytes, st, sp);
     if (const int rc = check_launch("xg_kv4_attention")) return rc;
     if (!sp.split) return XG_OK;
-    launch(kv4_combine_kernel<T, D, NT>, (unsigned)grid, 1024, 0, st, sp, grid);
+    launch(kv4_combine_kernel<T, D, NT>, (unsigned)grid, kCombineThreads, 0, st, sp, grid);
     return check_launch("xg_kv4_attention");
 }
 
