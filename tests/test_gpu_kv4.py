@@ -440,13 +440,12 @@ def test_refusals(cuda_device):
 
 # ---- together ----------------------------------------------------------------------------------------
 def _step(x, weights, cache, table, lens, starts, max_q, slots, positions, tables, heads, kv_heads, d):
-    from xpu_graph_b200 import ops
+    from xpu_graph_b200 import modules, ops
 
     w_qkv, w_o, wq, wk = weights
     qkv = ops.dense(x, w_qkv, True, None, None, "none").view(len(x), heads + 2 * kv_heads, d)
-    q, k = ops.qk_norm_rope(qkv[:, :heads], qkv[:, heads:heads + kv_heads], wq, wk, 1e-6, *tables, positions, [])
-    ops.kv4_append(cache, k, qkv[:, heads + kv_heads:], slots)
-    a = ops.kv4_attention(q, cache, table, lens, starts, max_q, d ** -0.5)
+    q, k = modules.QKNormRopeModule()(qkv[:, :heads], qkv[:, heads:heads + kv_heads], wq, wk, 1e-6, *tables, positions)
+    a = modules.CachedAttentionModule()(q, k, qkv[:, heads + kv_heads:], cache, slots, table, lens, starts, max_q)
     return ops.dense(a.flatten(1), w_o, True, None, None, "none")
 
 
@@ -508,6 +507,41 @@ def test_serving_steps(cuda_device):
     assert ((got.float() - want.float()).norm() / want.float().norm()).item() < 0.03
     k, f = (ops.kv4_read(c, slots, torch.float32)[0] for c in (cache, filled))
     assert ((k - f).norm() / f.norm()).item() < 0.03
+
+
+def test_sequences_that_fork_and_move(cuda_device):
+    """KV4Cache with the operators: forks that go on apart, frees and a compaction leave every sequence's attention as it is."""
+    from xpu_graph_b200 import ops
+    from xpu_graph_b200.kv_cache import KV4Cache
+
+    dev, heads, d = cuda_device, 2, 64
+    cache = KV4Cache(40, heads, d, page_size=32, device=dev)
+    g = torch.Generator(dev).manual_seed(0)
+
+    def grow(seq, n):
+        k, v = (torch.randn(n, heads, d, generator=g, device=dev) for _ in range(2))
+        ops.kv4_append(cache.layers[0], k, v, cache.extend(seq, n))
+
+    seqs = [cache.new() for _ in range(3)]
+    for seq, n in zip(seqs, (100, 64, 7)):
+        grow(seq, n)
+    seqs += [cache.fork(seqs[0]), cache.fork(seqs[1]), cache.fork(seqs[2])]
+    for i, seq in enumerate(seqs):
+        grow(seq, 3 + i)
+    q = torch.randn(len(seqs), 4, d, generator=g, device=dev).bfloat16()
+
+    def attend(which):
+        table, lens = cache.tables([seqs[i] for i in which])
+        return ops.kv4_attention(q[which], cache.layers[0], table, lens, None, 1, d ** -0.5)
+
+    before = attend([0, 1, 2, 3, 4, 5])
+    assert not torch.equal(before[0], before[3])
+    cache.free(seqs[1])
+    cache.free(seqs[0])
+    assert cache.compact() + cache.free_pages == 40
+    # (other sequences beside it, other cuts: roundings of fp16 times half a range of 3, and a bf16 step)
+    after = attend([2, 3, 4, 5]).float()
+    assert ((after - before[2:].float()).abs() <= 2.0 ** -11 * 6 + 2.0 ** -7 * after.abs()).all()
 
 
 def test_operators_compile(cuda_device):

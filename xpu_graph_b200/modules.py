@@ -208,6 +208,28 @@ class SDPAModule(torch.nn.Module):
         return _X.sdpa(q, k, v, attn_mask, float(scale), bool(is_causal))
 
 
+# ---- serving from a 4-bit cache --------------------------------------------------------------
+class QKNormRopeModule(torch.nn.Module):
+    """RMSNorm of every query and key head and the rotary embedding in one pass: forward(q, k, q_weight, k_weight, epsilon, cos,
+    sin, positions, sections) -> (q, k). q, k: [tokens, heads, D], slices of a packed projection as they are; a weight of None
+    leaves its tensor unnormalised; positions [tokens], or [axes, tokens] with the frequency pairs of each axis in `sections`."""
+
+    def forward(self, q, k, q_weight, k_weight, epsilon, cos, sin, positions, sections=()):
+        q, k = _X.qk_norm_rope(q, k, q_weight, k_weight, float(epsilon), cos, sin, positions, [int(n) for n in sections])
+        return q, k
+
+
+class CachedAttentionModule(torch.nn.Module):
+    """One layer's step over a 4-bit cache: the new tokens' keys and values go into `slots`, then the queries see everything that
+    their sequences hold. forward(q, k, v, cache, slots, page_table, kv_lens, q_starts, max_q, scale) -> [tokens, heads, D]."""
+
+    def forward(self, q, k, v, cache, slots, page_table, kv_lens, q_starts=None, max_q=1, scale=None):
+        _X.kv4_append(cache, k, v, slots)
+        if scale is None:
+            scale = q.shape[-1] ** -0.5
+        return _X.kv4_attention(q, cache, page_table, kv_lens, q_starts, max_q, float(scale))
+
+
 # ---- copy fusions --------------------------------------------------------------------------
 class FuseSliceModule(torch.nn.Module):
     """FusedSlice target (structure/fuse_slice.py:96-106): ``M(start_indices)``;
