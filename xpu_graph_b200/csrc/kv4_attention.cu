@@ -760,7 +760,7 @@ int launch_split(SplitParams sp, cudaStream_t st) {
     if (!reserve_smem(kv4_split_kernel<T, D, NT>, Cfg::smem(kMaxBatch), reserved)) return fail(XG_ERR_LAUNCH, "xg_kv4_attention: cannot reserve shared memory");
     const int bytes = Cfg::smem(sp.a.batch), fit = kSmSharedBytes / (bytes + 1024);
     const int grid = num_sms() * (fit < Cfg::CTAS ? fit : Cfg::CTAS);  // all resident
-    launch_with({.early = false}, kv4_split_kernel<T, D, NT>, (unsigned)grid, kWarps * 32, (size_t)bytes, st, sp);
+    launch(kv4_split_kernel<T, D, NT>, (unsigned)grid, kWarps * 32, (size_t)bytes, st, sp);
     if (const int rc = check_launch("xg_kv4_attention")) return rc;
     if (!sp.split) return XG_OK;
     launch(kv4_combine_kernel<T, D, NT>, (unsigned)grid, kCombineThreads, 0, st, sp, grid);
@@ -860,6 +860,7 @@ extern "C" int xg_kv4_attention(const void* q, const void* cache, int64_t pages,
     if (tokens < 0 || batch < 0 || q_heads <= 0 || q_heads % kv_heads != 0 || max_q < 0 || table_pages < 0 || workspace_bytes < 0)
         return fail(XG_ERR_INVALID_ARG, "xg_kv4_attention: bad extents");
     if (q_heads > 65535 || batch > 0x7fffff || tokens > 0x7fffffff || table_pages > 0x7ffffff) return fail(XG_ERR_TOO_LARGE, "xg_kv4_attention: extents");
+    if (tokens * (q_heads / kv_heads) > 0x7fffff00LL) return fail(XG_ERR_TOO_LARGE, "xg_kv4_attention: 2^31 rows per kv head or more");
     if (table_pages * page_size > 0x7fffff00LL) return fail(XG_ERR_TOO_LARGE, "xg_kv4_attention: more than 2^31 tokens per sequence");
     if (tokens == 0) return XG_OK;
     if (!q || !out || (batch > 0 && (!kv_lens || (table_pages > 0 && !page_table)))) return fail(XG_ERR_INVALID_ARG, "xg_kv4_attention: null pointer");

@@ -212,7 +212,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
             }
         };
         for (int j = 0; j < STAGES; ++j) issue(j);
-        const __half2 zero = __half2half2(__ushort_as_half(0));
+        // A NaN among a token's values reaches the rows that see it through their scores, and no other row.
+        const __half2 zero = __half2half2(__ushort_as_half(0)), lowest = __half2half2(__ushort_as_half(0xfbff));
         bool ok = true;
         // keys: a lane takes chunk t of rows r and r + 8; the bits are dealt so that neither its reads nor its swizzled writes collide
         const int kr = (lane & 1) | ((lane >> 3) & 1) << 1 | ((lane >> 1) & 1) << 2, kt = ((lane >> 4) & 1) | ((lane >> 2) & 1) << 1;
@@ -233,9 +234,12 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
                 for (int half = 0; half < Cfg::TOKENS / 8; ++half) {
                     const int r = kr + 8 * half;
                     uint32_t words[W];
-                    __half2 pairs[GR];
+                    __half2 pairs[GR], v_pairs[GR];
                     load_words<W>(codes + r * (D / 2) + kt * (D / 8), words);
                     load_pairs<GR>(pair_s + r * (D / 16), pairs);
+                    load_pairs<GR>(pair_s + P + r * (D / 16), v_pairs);
+#pragma unroll
+                    for (int gr = 0; gr < GR; ++gr) pairs[0] = __hfma2(v_pairs[gr], zero, pairs[0]);  // NaN if the token's values hold one
 #pragma unroll
                     for (int gr = 0; gr < GR; ++gr) {
                         const __half2 pair = r < there ? pairs[gr] : zero, scale = __low2half2(pair), least = __high2half2(pair);
@@ -262,7 +266,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
                     load_pairs<GR>(pair_s + P + r * (D / 16), pairs);
 #pragma unroll
                     for (int w = 0; w < GR; ++w) {
-                        const __half2 pair = r < there ? pairs[w] : zero;
+                        // (a NaN, with codes of 0, becomes finite: a product with the probability 0 of a row that does not see it is 0)
+                        const __half2 pair = r < there ? __hmax2(pairs[w], lowest) : zero;
                         ptx::st_shared_v4(base + (uint32_t)(w * (PN * 128) + r * 128 + ((chunk ^ (r & 7)) << 4)),
                                           unpack8(words[w], __low2half2(pair), __high2half2(pair)));
                     }
@@ -614,7 +619,7 @@ int launch_prefill(const AttendParams& p, int beyond, void* workspace, cudaStrea
         parts.ml = reinterpret_cast<float2*>(parts.rows + rows * D);
         parts.unit = reinterpret_cast<Unit*>(parts.ml + rows);
     }
-    launch_with({.early = false}, kv4_prefill_kernel<T, D>, (unsigned)(units * parts.splits), kPrefillThreads, Cfg::SMEM, st, p, beyond, parts);
+    launch(kv4_prefill_kernel<T, D>, (unsigned)(units * parts.splits), kPrefillThreads, Cfg::SMEM, st, p, beyond, parts);
     if (const int rc = check_launch("xg_kv4_attention")) return rc;
     if (parts.splits == 1) return XG_OK;
     launch(kv4_prefill_combine_kernel<T, D>, dim3((unsigned)units, Cfg::ROWS / 8), 256, 0, st, p, parts);

@@ -22,8 +22,7 @@ namespace xg {
 namespace kv4 {
 
 constexpr int kTileTokens = 16;
-constexpr int kGroup = 64;               // channels per scale
-constexpr float kLargest = 65504.0f;     // of fp16: values beyond are held as it
+constexpr float kLargest = 65504.0f;  // of fp16: values beyond are held as it
 
 __host__ __device__ constexpr int tile_bytes(int D) { return 18 * D; }
 
