@@ -767,8 +767,10 @@ int launch_split(SplitParams sp, cudaStream_t st) {
     return check_launch("xg_kv4_attention");
 }
 
-// Columns per unit: what the sequences bring, 16 where they bring more than 8. D = 256 has no registers for 16.
-constexpr int columns(int64_t D, int64_t max_q, int64_t group) { return D == 256 || max_q * group <= 8 ? 8 : 16; }
+// Columns per unit: what the sequences bring, 16 where they bring more than 8, but three units of 8 rather than two of 16 where that
+// holds them (8 sequences of 8192 to 16384, 8 kv heads of 128, 24 columns: 84 us, with two of 16 90; 16 columns in one of 16 55 us, in
+// two of 8 63). D = 256 has no registers for 16.
+constexpr int columns(int64_t D, int64_t max_q, int64_t group) { return D == 256 || max_q * group <= 8 || (max_q * group + 7) / 8 == 3 ? 8 : 16; }
 
 // Whether units are cut over CTAs. Left whole, they need no second launch.
 bool cut(int64_t D, int64_t cols, int64_t units, int64_t max_len) {
