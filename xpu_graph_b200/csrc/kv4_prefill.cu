@@ -129,32 +129,44 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
     if (warp == UNPACK) ptx::tmem_alloc(tmem_slot, 512);
     pdl_sync();
     if (warp == 0) {  // which rows are this CTA's: the sequences' units one after the other, the last rows (most keys) first
-        int base = 0;
-        Unit u = {};
-        for (int b0 = 0; b0 < p.batch; b0 += 32) {
-            const int b = b0 + lane;
-            Sequence s = {};
-            int w = 0;
-            if (b < p.batch) {
-                s = sequence(p, b);
-                if (s.count * p.group > beyond) w = (s.count * p.group + Cfg::ROWS - 1) / Cfg::ROWS * p.cache.heads;
+        constexpr int K = 4;  // sequences per lane: their loads overlap
+        const uint32_t mine = blockIdx.x / parts.splits;
+        uint32_t base = 0;
+        bool found = false;
+        for (int b0 = 0; b0 < p.batch && !found; b0 += 32 * K) {
+            Sequence s[K];
+            uint32_t w[K], sum = 0;
+#pragma unroll
+            for (int i = 0; i < K; ++i) {
+                const int b = b0 + lane * K + i;
+                s[i] = {};
+                if (b < p.batch) s[i] = sequence(p, b);
+                w[i] = s[i].count * p.group > beyond ? (uint32_t)((s[i].count * p.group + Cfg::ROWS - 1) / Cfg::ROWS) * p.cache.heads : 0;
+                sum += w[i];
             }
-            int inc = w;
+            uint32_t inc = sum;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(0xffffffffu, inc, o);
+                const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
                 if (lane >= o) inc += v;
             }
-            const int at = (int)blockIdx.x / parts.splits - base;
-            if (at >= inc - w && at < inc) {
-                const int off = at - (inc - w), tiles = w / p.cache.heads;
-                u = {1, b, off % p.cache.heads, tiles - 1 - off / p.cache.heads, (int)s.first, s.count, (int)s.len, 0};
-                *unit = u;
+            uint32_t off = mine - base - (inc - sum);  // of this lane's units
+            const uint32_t here = __ballot_sync(0xffffffffu, off < sum);
+            found = here != 0;
+            if (found && lane == __ffs(here) - 1) {  // (one lane, whatever q_starts holds)
+#pragma unroll
+                for (int i = 0; i < K; ++i) {
+                    if (off < w[i]) {
+                        const int tiles = (int)(w[i] / p.cache.heads);
+                        *unit = {1, b0 + lane * K + i, (int)(off % p.cache.heads), tiles - 1 - (int)(off / p.cache.heads), (int)s[i].first, s[i].count, (int)s[i].len, 0};
+                        break;
+                    }
+                    off -= w[i];
+                }
             }
-            if (__any_sync(0xffffffffu, u.on)) break;
             base += __shfl_sync(0xffffffffu, inc, 31);
         }
-        if (!__any_sync(0xffffffffu, u.on) && lane == 0) *unit = {};
+        if (!found && lane == 0) *unit = {};
     }
     ptx::tc_fence_before();
     __syncthreads();
