@@ -383,12 +383,13 @@ int xg_copy_pages(void* base, int64_t pages, int64_t page_bytes, int64_t page_st
 /*
  * Attention of the newest tokens of every sequence over its pages: out = softmax(q k^T * scale) v.
  * q: [tokens, q_heads, D] by element strides per token and head; out: contiguous. Rows q_starts[b] .. q_starts[b+1] (device,
- * batch + 1 entries; null: row b alone) belong to sequence b, whose kv_lens[b] cached tokens include them: of its n rows, row i
- * sees the keys up to position kv_lens[b] - n + i. max_q: the most rows that a sequence has; the results do not depend on it, the
- * choice of the kernel does. Token j of
- * sequence b lies in page page_table[b * table_stride + j / page_size]; a page number outside the cache hides its keys. q_heads is
- * a multiple of kv_heads, query head h reads kv head h / (q_heads / kv_heads). Rows that see no key, and rows of no sequence, are
- * zeros. 16-bit dtypes. All index arrays are int64 device memory. Workspace: xg_kv4_attention_workspace_bytes (max_len =
+ * batch + 1 non-decreasing entries; null: row b alone) belong to sequence b, whose kv_lens[b] cached tokens include them: of its n
+ * rows, row i sees the keys up to position kv_lens[b] - n + i. max_q: the most rows that a sequence has; it chooses the kernels (the
+ * results are within rounding of each other, and any value is safe). Token j of sequence b lies in page page_table[b * table_stride +
+ * j / page_size]; a page number outside the cache hides its keys. q_heads is a multiple of kv_heads, query head h reads kv head
+ * h / (q_heads / kv_heads). Rows that see no key, and rows of no sequence, are zeros; a NaN in a key or a value makes NaN of the rows
+ * that see it, and of no other. 16-bit dtypes. All index arrays are int64 device memory; lengths and starts out of range are clamped
+ * to what there is (rows that starts going back leave out, or give twice, are unspecified). Workspace: xg_kv4_attention_workspace_bytes (max_len =
  * table_pages * page_size), 16-byte aligned; its contents before and after the call are unspecified.
  * Reference counterpart: the same aten.scaled_dot_product_attention call site as xg_sdpa_fwd, for a cache it does not have.
  */

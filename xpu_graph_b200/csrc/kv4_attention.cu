@@ -37,7 +37,10 @@ using namespace kv4;
 // The codes of keys that do not exist are finite whatever they are; their scales are replaced, not multiplied away.
 //
 // Code that runs once per unit is kept short: fetching it costs more than running it (with a second copy of the loop for masked
-// blocks 64 sequences of 512 to 8192 tokens took 92 us, and of 4096 each 78).
+// blocks 64 sequences of 512 to 8192 tokens took 92 us, with one 82).
+// What bounds it: unpacking and the softmax's scalar work, 54 % of the issue slots and 48 % of the logic pipe at three warps a
+// scheduler, beside 50 % of HBM: 4 sequences of 65536, 32 / 8 heads of 128: 75 us, 4.05 TB/s (the loads alone 60, the arithmetic alone
+// 73). More tiles in work at once, other occupancies, packed fp32 pairs and shifts by multiplication gave nothing.
 constexpr int kWarps = 4;
 constexpr int kBlockTiles = 2, kBlockKeys = kBlockTiles * kTileTokens;  // what a stage holds
 constexpr int kMaxBatch = 1024;  // sequences per launch: their prefix sums live in shared memory
@@ -117,7 +120,7 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
         ptx::fence_mbar_init();
         ptx::fence_proxy_async();
     }
-    pdl_sync();
+    pdl_wait();
 
     // ---- the line of tiles
     const int kv_heads = p.cache.heads;
@@ -622,6 +625,9 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
     __syncthreads();
     if (*abort_flag) ok = false;
 
+    // (Not earlier: with the next kernel's CTAs waiting in the places of those that are through, 256 sequences of 16 to 1000 took 83 us
+    // instead of 74.)
+    pdl_trigger();
     // ---- what the warps' cuts left: heads that belong to an earlier CTA's unit, then every tail with the heads behind it
     for (int a = -1; a < kWarps && ok; ++a) {
         if (a >= 0 && !cut_s[a].tail) continue;
@@ -772,7 +778,8 @@ int launch_split(SplitParams sp, cudaStream_t st) {
 // two of 8 63). D = 256 has no registers for 16.
 constexpr int columns(int64_t D, int64_t max_q, int64_t group) { return D == 256 || max_q * group <= 8 || (max_q * group + 7) / 8 == 3 ? 8 : 16; }
 
-// Whether units are cut over CTAs. Left whole, they need no second launch.
+// Whether units are cut over CTAs. Left whole, they need no second launch, but the CTAs' loads differ by a unit. (us, whole / cut, 32 / 8
+// heads of 128) 1 sequence of 512 11.0 / 11.8, 512 of 512 83 / 86, 256 of 16 to 1000 69 / 74; 64 of 1024 34 / 32, 128 of 1400 66 / 59.
 bool cut(int64_t D, int64_t cols, int64_t units, int64_t max_len) {
     return max_len > 1024 || (max_len > 512 && units < 2LL * num_sms() * split_ctas((int)D, (int)cols / 8));
 }
@@ -783,9 +790,9 @@ int64_t split_workspace(int64_t D, int64_t max_q, int64_t group, int64_t max_len
     return 2 * ctas * cols * (D + 2) * 4 + ctas * (int64_t)sizeof(PartDesc);
 }
 
-// Sequences with more columns (new token, head of the group) than this go to the tensor-memory kernel.
-// Streaming unpacks the keys once per 16 columns, the other once per 256: (us, streamed / tiles, 32/8 heads of 128) 8 sequences of 4096,
-// 48 columns 54 / 57; of 8192, 64 columns 111 / 94; of 4096, 120 columns 109 / 90; 1 of 8192, 64 columns 31 / 32.
+// Sequences with more columns (new token, head of the group) than this go to the tensor-memory kernel: streaming unpacks the keys once
+// per 16 columns, the other once per 256. (us, streamed / tiles, 32 / 8 heads of 128) 8 sequences of 4096, 48 columns 54 / 57; of 8192,
+// 64 columns 111 / 94; of 4096, 120 columns 109 / 90; 1 of 8192, 64 columns 31 / 32.
 constexpr int kMostStreamed = 48;
 constexpr bool in_tiles(int64_t max_q, int64_t group) { return max_q * group > kMostStreamed; }
 

@@ -10,7 +10,12 @@
 // probabilities; fp16 queries stay as they are and bf16 ones too, after a power of two per row has been taken out (it returns in the
 // row's exponent factor). Sums are fp32 in tensor memory and registers.
 //
-// What bounds it: unpacking 64 keys (2 operations per code) and 256 x 64 exponentials run beside 1024 cycles of products per block.
+// What bounds it: per block of 64 keys the products take 1024 cycles of the tensor pipe (38 % busy), the 256 x 64 exponentials 1024 of
+// the special-function unit (39 %), and unpacking (2 operations per code) and softmax 48 % of the issue slots; they run beside each
+// other, but a tile's scores, probabilities and product follow one another. 3 sequences of 2048 to 8192 keys with 2048 new tokens, 32 /
+// 8 heads of 128: 0.53-0.58 ms, 840-920 TFLOP/s (without unpacking 0.45). Tried without gain: a warpgroup more for unpacking with the
+// registers dealt out anew; the last wave's units shared out over the idle CTAs (their parts cost what the wave gains). Head dim 256
+// has room for one tile and one buffer of V: 500 TFLOP/s.
 #include "kv4_attend.cuh"
 
 namespace xg {
@@ -53,7 +58,7 @@ struct Parts {
     float* rows;  // [units][splits][256][D]
     float2* ml;   // [units][splits][256]
     Unit* unit;   // [units]
-    int splits;   // 1: none of this
+    int splits;   // 1: none of this. 128 new tokens behind 32640, 32 / 8 heads: 105 us, one CTA per unit 650
 };
 
 // 8 codes as fp16 values, in the order 0 4 1 5 2 6 3 7, in which masks find them: q lies in that order too, and the output's columns
