@@ -376,13 +376,24 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
             // this row of q, a power of two taken out, into the operand tile
             const T* q = reinterpret_cast<const T*>(p.q) + (int64_t)(u.first + token) * p.q_st + (int64_t)head * p.q_sh;
             const bool vec = (reinterpret_cast<uintptr_t>(p.q) & 15) == 0 && p.q_st % 8 == 0 && p.q_sh % 8 == 0;
+            // (the whole row in registers where it fits, so that one latency is paid: 16 rounds of loads cost as much as four blocks)
+            constexpr int HELD = D <= 128 ? D / 8 : 1;
+            uint4 held[HELD];
+            auto piece = [&](int c) { return there ? load_q8(q + 8 * c, vec) : make_uint4(0, 0, 0, 0); };
             float top = 0.f;
-#pragma unroll 4
-            for (int c = 0; c < D / 8; ++c) {
-                const uint4 raw = there ? load_q8(q + 8 * c, vec) : make_uint4(0, 0, 0, 0);
+            auto take = [&](const uint4& raw) {
                 const T* e = reinterpret_cast<const T*>(&raw);
 #pragma unroll
                 for (int x = 0; x < 8; ++x) top = fmaxf(top, fabsf(Cvt<T>::to_f(e[x])));
+            };
+            if (D <= 128) {
+#pragma unroll
+                for (int c = 0; c < HELD; ++c) held[c] = piece(c);
+#pragma unroll
+                for (int c = 0; c < HELD; ++c) take(held[c]);
+            } else {
+#pragma unroll 8
+                for (int c = 0; c < D / 8; ++c) take(piece(c));
             }
             int e = (int)(__float_as_uint(top) >> 23) - 127;
             e = max(-100, min(126, e));
@@ -391,14 +402,19 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
             if (p.scale < 0.f) down = -down;
             mul = fmaxf((p.scale == 0.f ? 1.f : fabsf(p.scale)) * kLog2e * __uint_as_float((uint32_t)(127 + e) << 23), 1e-37f);
             const uint32_t base = ptx::smem_u32(q_s + i * Cfg::Q_BYTES) + (uint32_t)(r_in_tile * 128);
-#pragma unroll 4
-            for (int c = 0; c < D / 8; ++c) {  // (the row once more, from the cache)
-                const uint4 raw = there ? load_q8(q + 8 * c, vec) : make_uint4(0, 0, 0, 0);
+            auto put = [&](int c, const uint4& raw) {
                 const T* e8 = reinterpret_cast<const T*>(&raw);
                 uint32_t w[4];
 #pragma unroll
                 for (int x = 0; x < 4; ++x) w[x] = ptx::pack2<__half>(Cvt<T>::to_f(e8[x]) * down, Cvt<T>::to_f(e8[x + 4]) * down);  // (unpack8's order)
                 ptx::st_shared_v4(base + (uint32_t)((c >> 3) * (PM * 128) + (((c & 7) ^ (r_in_tile & 7)) << 4)), make_uint4(w[0], w[1], w[2], w[3]));
+            };
+            if (D <= 128) {
+#pragma unroll
+                for (int c = 0; c < HELD; ++c) put(c, held[c]);
+            } else {
+#pragma unroll 8
+                for (int c = 0; c < D / 8; ++c) put(c, piece(c));  // (the row once more, from the cache)
             }
             ptx::fence_proxy_async();
             ptx::mbar_arrive(&q_full[i]);
