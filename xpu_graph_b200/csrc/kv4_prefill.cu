@@ -376,24 +376,25 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
             // this row of q, a power of two taken out, into the operand tile
             const T* q = reinterpret_cast<const T*>(p.q) + (int64_t)(u.first + token) * p.q_st + (int64_t)head * p.q_sh;
             const bool vec = (reinterpret_cast<uintptr_t>(p.q) & 15) == 0 && p.q_st % 8 == 0 && p.q_sh % 8 == 0;
-            // (the whole row in registers where it fits, so that one latency is paid: 16 rounds of loads cost as much as four blocks)
-            constexpr int HELD = D <= 128 ? D / 8 : 1;
+            // 16 loads at once, a row of 128 (what stands in front of a unit's first block counts: four at a time, and again for the second
+            // use, 3 sequences with 2048 new tokens took 505 us where this takes 475, 600 with 20 each 733 and now 572); of a row of 256 the
+            // first half comes a second time, from the cache. A row per group of lanes, with whole lines per load, took 497 and 679.
+            constexpr int HELD = D < 128 ? D / 8 : 16;
             uint4 held[HELD];
-            auto piece = [&](int c) { return there ? load_q8(q + 8 * c, vec) : make_uint4(0, 0, 0, 0); };
-            float top = 0.f;
-            auto take = [&](const uint4& raw) {
-                const T* e = reinterpret_cast<const T*>(&raw);
+            auto fetch = [&](int c0) {
 #pragma unroll
-                for (int x = 0; x < 8; ++x) top = fmaxf(top, fabsf(Cvt<T>::to_f(e[x])));
+                for (int c = 0; c < HELD; ++c) held[c] = there ? load_q8(q + 8 * (c0 + c), vec) : make_uint4(0, 0, 0, 0);
             };
-            if (D <= 128) {
+            float top = 0.f;
 #pragma unroll
-                for (int c = 0; c < HELD; ++c) held[c] = piece(c);
+            for (int c0 = 0; c0 < D / 8; c0 += HELD) {
+                fetch(c0);
 #pragma unroll
-                for (int c = 0; c < HELD; ++c) take(held[c]);
-            } else {
-#pragma unroll 8
-                for (int c = 0; c < D / 8; ++c) take(piece(c));
+                for (int c = 0; c < HELD; ++c) {
+                    const T* e = reinterpret_cast<const T*>(&held[c]);
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) top = fmaxf(top, fabsf(Cvt<T>::to_f(e[x])));
+                }
             }
             int e = (int)(__float_as_uint(top) >> 23) - 127;
             e = max(-100, min(126, e));
@@ -402,19 +403,18 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
             if (p.scale < 0.f) down = -down;
             mul = fmaxf((p.scale == 0.f ? 1.f : fabsf(p.scale)) * kLog2e * __uint_as_float((uint32_t)(127 + e) << 23), 1e-37f);
             const uint32_t base = ptx::smem_u32(q_s + i * Cfg::Q_BYTES) + (uint32_t)(r_in_tile * 128);
-            auto put = [&](int c, const uint4& raw) {
-                const T* e8 = reinterpret_cast<const T*>(&raw);
-                uint32_t w[4];
 #pragma unroll
-                for (int x = 0; x < 4; ++x) w[x] = ptx::pack2<__half>(Cvt<T>::to_f(e8[x]) * down, Cvt<T>::to_f(e8[x + 4]) * down);  // (unpack8's order)
-                ptx::st_shared_v4(base + (uint32_t)((c >> 3) * (PM * 128) + (((c & 7) ^ (r_in_tile & 7)) << 4)), make_uint4(w[0], w[1], w[2], w[3]));
-            };
-            if (D <= 128) {
+            for (int c0 = D / 8 - HELD; c0 >= 0; c0 -= HELD) {
+                if (c0 != D / 8 - HELD) fetch(c0);
 #pragma unroll
-                for (int c = 0; c < HELD; ++c) put(c, held[c]);
-            } else {
-#pragma unroll 8
-                for (int c = 0; c < D / 8; ++c) put(c, piece(c));  // (the row once more, from the cache)
+                for (int c = 0; c < HELD; ++c) {
+                    const T* e8 = reinterpret_cast<const T*>(&held[c]);
+                    uint32_t w[4];
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) w[x] = ptx::pack2<__half>(Cvt<T>::to_f(e8[x]) * down, Cvt<T>::to_f(e8[x + 4]) * down);  // (unpack8's order)
+                    const int at = c0 + c;
+                    ptx::st_shared_v4(base + (uint32_t)((at >> 3) * (PM * 128) + (((at & 7) ^ (r_in_tile & 7)) << 4)), make_uint4(w[0], w[1], w[2], w[3]));
+                }
             }
             ptx::fence_proxy_async();
             ptx::mbar_arrive(&q_full[i]);
