@@ -120,6 +120,8 @@ def test_lengths_and_starts_out_of_range(cuda_device):
         assert torch.equal(got, want)
         for starts in ([5, 3, 90], [-7, 100, 2], [200, 300, 400]):
             assert ops.kv4_attention(q, cache, table, lens, _dev(starts, cuda_device), most, 0.1).shape == q.shape
+    # no sequence at all
+    assert not ops.kv4_attention(q, cache, table[:0], lens[:0], lens.new_zeros(1), 100, 0.1).any()
     torch.cuda.synchronize()
     assert lib.tc_status() == 0
 

@@ -10,12 +10,12 @@
 // probabilities; fp16 queries stay as they are and bf16 ones too, after a power of two per row has been taken out (it returns in the
 // row's exponent factor). Sums are fp32 in tensor memory and registers.
 //
-// What bounds it: per block of 64 keys the products take 1024 cycles of the tensor pipe (38 % busy), the 256 x 64 exponentials 1024 of
-// the special-function unit (39 %), and unpacking (2 operations per code) and softmax 48 % of the issue slots; they run beside each
-// other, but a tile's scores, probabilities and product follow one another. 3 sequences of 2048 to 8192 keys with 2048 new tokens, 32 /
-// 8 heads of 128: 0.53-0.58 ms, 840-920 TFLOP/s (without unpacking 0.45). Tried without gain: a warpgroup more for unpacking with the
+// What bounds it: per block of 64 keys the products take 1024 cycles of the tensor pipe (41 % busy), the 256 x 64 exponentials 1024 of
+// the special-function unit (41 %), and unpacking (2 operations per code) and softmax 49 % of the issue slots; they run beside each
+// other, but a tile's scores, probabilities and product follow one another, and about 8 us in front of and behind a unit's blocks
+// overlap with nothing. 3 sequences of 2048 to 8192 keys with 2048 new tokens, 32 / 8 heads of 128: 0.475-0.49 ms, 990-1024 TFLOP/s. Tried without gain: a warpgroup more for unpacking with the
 // registers dealt out anew; the last wave's units shared out over the idle CTAs (their parts cost what the wave gains). Head dim 256
-// has room for one tile and one buffer of V: 500 TFLOP/s.
+// has room for one tile and one buffer of V: 566 TFLOP/s.
 #include "kv4_attend.cuh"
 
 namespace xg {
