@@ -126,6 +126,21 @@ def test_lengths_and_starts_out_of_range(cuda_device):
     assert lib.tc_status() == 0
 
 
+@pytest.mark.parametrize("d,group", [(64, 1), (128, 4), (256, 2)])
+def test_one_sequence_with_rows_around_it(cuda_device, d, group):
+    """However many of the rows are the sequence's, and whatever the hint says: its rows attend, the others are zeros."""
+    from xpu_graph_b200 import lib, ops
+
+    cache = _filled(60, 2, 32, d, cuda_device)
+    table = _table([1700], 32, 60, cuda_device)
+    q = torch.randn(300, 2 * group, d, generator=torch.Generator().manual_seed(d)).half().to(cuda_device)
+    for n, lo, hi, most in ((1700, 5, 290, 300), (1700, 0, 300, 300), (333, 298, 300, 300), (90, 7, 8, 4000), (40, 10, 130, 120), (0, 3, 200, 300), (64, 9, 9, 300), (1700, 100, 300, 1)):
+        got = ops.kv4_attention(q, cache, table, _dev([n], cuda_device), _dev([lo, hi], cuda_device), most, d ** -0.5)
+        _check_attention(got, _reference(q, cache, table, [n], [lo, hi], d ** -0.5), f"{n} {lo} {hi} {most}", halves=most > 8)
+        assert not got[:lo].any() and not got[hi:].any()
+    assert lib.tc_status() == 0
+
+
 def test_gradients_are_refused(cuda_device):
     """Serving operators: inputs that need a gradient run, going back through them does not."""
     from xpu_graph_b200 import ops

@@ -108,7 +108,8 @@ __device__ __forceinline__ int64_t tile_of_token(const AttendParams& p, int b, i
 
 }  // namespace kv4
 
-// Many new tokens per sequence (kv4_prefill.cu): the sequences with more than `beyond` columns (new token, head of the group).
+// Many new tokens per sequence (kv4_prefill.cu): the sequences with more than `beyond` columns (new token, head of the group); with
+// `beyond` 0 and one sequence also the rows of none.
 int attend_prefill(const kv4::AttendParams& p, int64_t D, int dtype, int beyond, void* workspace, cudaStream_t st);
 int64_t prefill_workspace(int64_t tokens, int64_t batch, int64_t group, int64_t heads, int64_t D, int64_t max_len);
 int read_kv4_prefill_status(unsigned int* host_out, int reset);

@@ -172,6 +172,13 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
             base += __shfl_sync(0xffffffffu, inc, 31);
         }
         if (!found && lane == 0) *unit = {};
+    } else if (beyond == 0) {  // one sequence: the rows in front of it and behind it
+        const Sequence s = sequence(p, 0);
+        const int64_t per_row = (int64_t)p.heads * D;
+        for (int64_t r = blockIdx.x; r < p.tokens - s.count; r += gridDim.x) {
+            T* row = reinterpret_cast<T*>(p.out) + (r < s.first ? r : r + s.count) * per_row;
+            for (int64_t c = threadIdx.x - 32; c < per_row / 8; c += kPrefillThreads - 32) *reinterpret_cast<uint4*>(row + c * 8) = make_uint4(0, 0, 0, 0);
+        }
     }
     ptx::tc_fence_before();
     __syncthreads();
