@@ -58,7 +58,7 @@ struct Parts {
     float* rows;  // [units][splits][256][D]
     float2* ml;   // [units][splits][256]
     Unit* unit;   // [units]
-    int splits;   // 1: none of this. 128 new tokens behind 32640, 32 / 8 heads: 105 us, one CTA per unit 650
+    int splits;   // 1: none of this. 128 new tokens behind 32640, 32 / 8 heads: 98 us, one CTA per unit 650
 };
 
 // 8 codes as fp16 values, in the order 0 4 1 5 2 6 3 7, in which masks find them: q lies in that order too, and the output's columns
@@ -635,11 +635,12 @@ __global__ void __launch_bounds__(256) kv4_prefill_combine_kernel(const AttendPa
     for (int c = 0; c < C; ++c) out[c * 32 + ch] = Cvt<T>::from_f(o[c] * inv);
 }
 
-// The most units there can be, and over how many CTAs each one's keys are shared out: as many as fill the chip once, 512 keys or more each.
+// The most units there can be, and over how many CTAs each one's keys are shared out: as many as fill the chip once, 256 keys or more each
+// (1 sequence of 1000 with 256 new tokens: 23.9 us, with 512 or more 27.5; 128 or more gain nothing further).
 int64_t most_units(int64_t tokens, int64_t batch, int64_t group, int64_t heads, int64_t rows) { return (tokens * group + batch * (rows - 1)) / rows * heads; }
 int key_splits(int64_t units, int64_t max_len) {
     int64_t n = num_sms() / (units > 0 ? units : 1);
-    if (n > max_len / 512) n = max_len / 512;
+    if (n > max_len / 256) n = max_len / 256;
     return (int)(n < 1 ? 1 : n);
 }
 

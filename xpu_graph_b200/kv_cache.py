@@ -85,11 +85,12 @@ class KV4Cache:
         return twin
 
     def free(self, seq: int) -> None:
+        """Ends a sequence. Its pages may go to the next one at once: kernels that read them are in front on the stream, or waited for."""
         self._drop(self._pages.pop(seq))
         del self._length[seq]
 
     def compact(self) -> int:
-        """Moves the pages in use to the front and returns how many they are."""
+        """Moves the pages in use to the front and returns how many they are. Slots and tables handed out before are stale."""
         used = [p for p, holders in enumerate(self._holders) if holders]
         gaps = [p for p, holders in enumerate(self._holders[:len(used)]) if not holders]
         src = [p for p in used if p >= len(used)]  # as many as there are gaps, and none of them one
