@@ -791,10 +791,11 @@ int64_t split_workspace(int64_t D, int64_t max_q, int64_t group, int64_t max_len
 }
 
 // Sequences with more columns (new token, head of the group) than this go to the tensor-memory kernel: streaming unpacks the keys once
-// per 16 columns, the other once per 256. (us, streamed / tiles, 32 / 8 heads of 128) 8 sequences of 4096, 48 columns 54 / 57; of 8192,
-// 64 columns 111 / 94; of 4096, 120 columns 109 / 90; 1 of 8192, 64 columns 31 / 32.
-constexpr int kMostStreamed = 48;
-constexpr bool in_tiles(int64_t max_q, int64_t group) { return max_q * group > kMostStreamed; }
+// per 16 columns (8 at head dim 256), the other once per 256 (128). (us, streamed / tiles, 8 kv heads) D = 128: 64 sequences of 4096, 32
+// columns 211 / 304, 36 307 / 303; 1 of 16000, 32 columns 31 / 32, 36 37 / 32. D = 64, where a tile's products are shorter than its
+// softmax: 64 of 4096, 64 columns 237 / 262, 72 291 / 260. D = 256: 32 of 2000, 48 columns 199 / 185, 1 of 16000, 48 63 / 61, 40 56 / 60.
+constexpr int most_streamed(int64_t D) { return D == 64 ? 64 : (D == 128 ? 32 : 40); }
+constexpr bool in_tiles(int64_t D, int64_t max_q, int64_t group) { return max_q * group > most_streamed(D); }
 
 template <typename T>
 int attend_split(const AttendParams& whole, int64_t D, int64_t max_q, int most_cols, void* workspace, cudaStream_t st) {
@@ -854,7 +855,7 @@ extern "C" int64_t xg_kv4_attention_workspace_bytes(int64_t tokens, int64_t batc
     using namespace xg;
     if (tokens <= 0 || batch <= 0 || q_heads <= 0 || kv_heads <= 0 || max_q < 0 || max_len < 0) return 0;
     const int64_t group = q_heads / kv_heads, streamed = split_workspace(D, max_q, group, max_len, batch, kv_heads);
-    const int64_t tiles = in_tiles(max_q, group) ? prefill_workspace(tokens, batch, group, kv_heads, D, max_len) : 0;
+    const int64_t tiles = in_tiles(D, max_q, group) ? prefill_workspace(tokens, batch, group, kv_heads, D, max_len) : 0;
     return streamed > tiles ? streamed : tiles;  // (used one after the other)
 }
 
@@ -886,9 +887,9 @@ extern "C" int xg_kv4_attention(const void* q, const void* cache, int64_t pages,
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     // Sequences with many columns go to the tensor-memory kernel, where there may be any; the others to the streaming one. A sequence
     // on its own goes there whatever it turns out to be, which saves the other's launches (512 new tokens: 20.6 us, with them 23.3).
-    const bool tiles = batch > 0 && in_tiles(max_q, p.group);
+    const bool tiles = batch > 0 && in_tiles(D, max_q, p.group);
     if (tiles && batch == 1) return attend_prefill(p, D, dtype, 0, workspace, st);
-    const int most = tiles ? kMostStreamed : 0x7fffffff;
+    const int most = tiles ? most_streamed(D) : 0x7fffffff;
     const int rc = dtype == XG_BF16 ? attend_split<__nv_bfloat16>(p, D, max_q, most, workspace, st) : attend_split<__half>(p, D, max_q, most, workspace, st);
     return rc != XG_OK || !tiles ? rc : attend_prefill(p, D, dtype, most, workspace, st);
 }

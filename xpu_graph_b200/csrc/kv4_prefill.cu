@@ -635,12 +635,16 @@ __global__ void __launch_bounds__(256) kv4_prefill_combine_kernel(const AttendPa
     for (int c = 0; c < C; ++c) out[c * 32 + ch] = Cvt<T>::from_f(o[c] * inv);
 }
 
-// The most units there can be, and over how many CTAs each one's keys are shared out: as many as fill the chip once, 256 keys or more each
-// (1 sequence of 1000 with 256 new tokens: 23.9 us, with 512 or more 27.5; 128 or more gain nothing further).
+// The most units there can be, and over how many CTAs each one's keys are shared out: as many as fill the chip once, 320 keys or more each
+// (1 sequence of 1000 with 256 new tokens: 25 us in three parts, whole 27.5; of 512, all new, 26 in two parts, whole 20.6).
 int64_t most_units(int64_t tokens, int64_t batch, int64_t group, int64_t heads, int64_t rows) { return (tokens * group + batch * (rows - 1)) / rows * heads; }
-int key_splits(int64_t units, int64_t max_len) {
+int key_splits(int64_t tokens, int64_t batch, int64_t group, int64_t heads, int64_t rows, int64_t max_len) {
+    // (how many units there are likely to be, with rows dealt out evenly: 8 sequences of 16000 with 9 new tokens, 8 heads of 256: two parts
+    // of 64 units 325 us; for the most there can be, 80, they stayed whole, 610)
+    const int64_t even = batch > 0 ? batch * (((tokens + batch - 1) / batch * group + rows - 1) / rows) * heads : 0;
+    const int64_t most = most_units(tokens, batch, group, heads, rows), units = even < most ? even : most;
     int64_t n = num_sms() / (units > 0 ? units : 1);
-    if (n > max_len / 256) n = max_len / 256;
+    if (n > max_len / 320) n = max_len / 320;
     return (int)(n < 1 ? 1 : n);
 }
 
@@ -652,7 +656,7 @@ int launch_prefill(const AttendParams& p, int beyond, void* workspace, cudaStrea
     // at least as many CTAs as there are units; those behind the last one return at once
     const int64_t units = most_units(p.tokens, p.batch, p.group, p.cache.heads, Cfg::ROWS);
     Parts parts = {};
-    parts.splits = key_splits(units, (int64_t)p.table_pages * p.cache.tiles * kTileTokens);
+    parts.splits = key_splits(p.tokens, p.batch, p.group, p.cache.heads, Cfg::ROWS, (int64_t)p.table_pages * p.cache.tiles * kTileTokens);
     if (units * parts.splits > 0x7fffffffLL) return fail(XG_ERR_TOO_LARGE, "xg_kv4_attention: too many rows");
     if (parts.splits > 1) {
         const int64_t rows = units * parts.splits * Cfg::ROWS;
@@ -671,7 +675,7 @@ int launch_prefill(const AttendParams& p, int beyond, void* workspace, cudaStrea
 
 int64_t prefill_workspace(int64_t tokens, int64_t batch, int64_t group, int64_t heads, int64_t D, int64_t max_len) {
     const int64_t rows = D == 256 ? PreCfg<256>::ROWS : PreCfg<128>::ROWS, units = most_units(tokens, batch, group, heads, rows);
-    const int splits = key_splits(units, max_len);
+    const int splits = key_splits(tokens, batch, group, heads, rows, max_len);
     return splits == 1 ? 0 : units * splits * rows * (D + 2) * 4 + units * (int64_t)sizeof(Unit);
 }
 
