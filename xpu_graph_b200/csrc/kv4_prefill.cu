@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
         ptx::fence_proxy_async();
     }
     if (warp == UNPACK) ptx::tmem_alloc(tmem_slot, 512);
-    pdl_sync();
+    pdl_wait();
     if (warp == 0) {  // which rows are this CTA's: the sequences' units one after the other, the last rows (most keys) first
         constexpr int K = 4;  // sequences per lane: their loads overlap
         const uint32_t mine = blockIdx.x / parts.splits;
@@ -183,6 +183,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
     ptx::tc_fence_before();
     __syncthreads();
     ptx::tc_fence_after();
+    pdl_trigger();  // the tensor memory is held
     const uint32_t tmem_base = *tmem_slot;
     const Unit u = *unit;
 
