@@ -383,7 +383,7 @@ int xg_copy_pages(void* base, int64_t pages, int64_t page_bytes, int64_t page_st
 /*
  * Attention of the newest tokens of every sequence over its pages: out = softmax(q k^T * scale) v.
  * q: [tokens, q_heads, D] by element strides per token and head; out: contiguous. Rows q_starts[b] .. q_starts[b+1] (device,
- * batch + 1 non-decreasing entries; null: row b alone) belong to sequence b, whose kv_lens[b] cached tokens include them: of its n
+ * batch + 1 non-decreasing entries; null: row b alone, and no more sequences than rows) belong to sequence b, whose kv_lens[b] cached tokens include them: of its n
  * rows, row i sees the keys up to position kv_lens[b] - n + i. max_q: the most rows that a sequence has; it chooses the kernels (the
  * results are within rounding of each other, and any value is safe). Token j of sequence b lies in page page_table[b * table_stride +
  * j / page_size]; a page number outside the cache hides its keys. q_heads is a multiple of kv_heads, query head h reads kv head

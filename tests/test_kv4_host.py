@@ -97,3 +97,17 @@ def test_page_lists():
         assert torch.equal(ops._host_ints(tuple(range(n))), torch.arange(n))
     with pytest.raises((RuntimeError, NotImplementedError)):
         ops.copy_pages(torch.zeros(2, 16), [0], [1])
+
+
+def test_a_row_for_each_sequence_where_there_are_no_starts():
+    """Without q_starts sequence b's row is row b: more sequences than rows are refused before any launch."""
+    L = lib.load()
+
+    def attend(tokens, batch, max_q):
+        need = L.xg_kv4_attention_workspace_bytes(tokens, batch, 4, 2, 64, max_q, 48)
+        return L.xg_kv4_attention(P, P, 2, 2, 16, 2 * 18 * 64, P, 3, 3, P, None, P, tokens, batch, 4, 64, max_q, 256, 64, 1.0, H, P, max(need, 0), None)
+
+    for tokens, batch, max_q in ((1, 2, 1), (1, 2, 100), (5, 4000, 1), (5, 4000, 100)):
+        assert attend(tokens, batch, max_q) == -1, (tokens, batch, max_q)
+        assert "row" in lib.last_error()
+    assert attend(0, 2, 1) == 0

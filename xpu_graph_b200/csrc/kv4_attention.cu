@@ -873,6 +873,8 @@ extern "C" int xg_kv4_attention(const void* q, const void* cache, int64_t pages,
     if (tokens * (q_heads / kv_heads) > 0x7fffff00LL) return fail(XG_ERR_TOO_LARGE, "xg_kv4_attention: 2^31 rows per kv head or more");
     if (table_pages * page_size > 0x7fffff00LL) return fail(XG_ERR_TOO_LARGE, "xg_kv4_attention: more than 2^31 tokens per sequence");
     if (tokens == 0) return XG_OK;
+    if (!q_starts && batch > tokens) return fail(XG_ERR_INVALID_ARG, "xg_kv4_attention: %lld sequences without q_starts need a row each, there are %lld",
+                                                 (long long)batch, (long long)tokens);
     if (!q || !out || (batch > 0 && (!kv_lens || (table_pages > 0 && !page_table)))) return fail(XG_ERR_INVALID_ARG, "xg_kv4_attention: null pointer");
     if (!aligned16(out)) return fail(XG_ERR_INVALID_ARG, "xg_kv4_attention: the result must be 16-byte aligned");
     AttendParams p = {};
