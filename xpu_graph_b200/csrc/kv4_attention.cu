@@ -445,13 +445,13 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
                     if (KT == 2) mx[nt][c] = ptx::fmax3(mx[nt][c], sc[KT - 1][nt][c], sc[KT - 1][nt][2 + c]);
                     grow = grow || mx[nt][c] > bar[nt][c];
                 }
-            __half2 v_top = __half2half2(__ushort_as_half(0));  // largest scale of the values (low half)
+            __half2 v_top = __half2half2(__ushort_as_half(0));  // largest scale of the values (low half; their size, should one be negative)
 #pragma unroll
             for (int k = 0; k < KT; ++k)
 #pragma unroll
                 for (int r = 0; r < 2; ++r)
 #pragma unroll
-                    for (int gr = 0; gr < GR; ++gr) v_top = __hmax2(v_top, vp[k][r][gr]);
+                    for (int gr = 0; gr < GR; ++gr) v_top = __hmax2(v_top, __habs2(vp[k][r][gr]));
             grow = grow || __hgt(__low2half(v_top), v_bar);
             if (__any_sync(0xffffffffu, grow)) {
                 float v_new = v_exp;

@@ -1,9 +1,10 @@
 // Keys and values in 4 bits: quantising new tokens into cache pages, reading tokens back, copying pages. All three move bytes and
 // are bound by HBM (the layout: kv4_tile.cuh).
 //
-// Quantising, per token, head and group of 64 channels: least = fp16(min x), scale = fp16((max x - least) * fp32(1/15)),
-// code = rint((x - least) / scale) in 0..15, every step in fp32 with IEEE rounding. The fp16 roundings of the pair come first,
-// so the codes are the nearest ones for the pair that is stored.
+// Quantising, per token, head and group of 64 channels: least = fp16(min x), scale = fp16(max(max x - least, 0) * fp32(1/15)),
+// code = rint((x - least) / scale) in 0..15 (0 where the scale is 0), every step in fp32 with IEEE rounding. The fp16 roundings of the
+// pair come first, so the codes are the nearest ones for the pair that is stored. (A least value that is rounded up beyond the largest
+// one has no range: a scale below 0 would be one that the attention, which bounds its weights by the scales, does not expect.)
 #include "kv4_tile.cuh"
 #include "sm100_ptx.cuh"
 
@@ -89,11 +90,11 @@ __device__ __forceinline__ void quantise(const Raw8<T> (&x)[2], uint32_t (&word)
     if (lo == lo) lo = fminf(fmaxf(lo, -kLargest), kLargest);
     const __half least = __float2half_rn(lo);
     const float least_f = __half2float(least);
-    const __half scale = __float2half_rn(__fmul_rn(hi - least_f, 1.0f / 15.0f));
+    const __half scale = __float2half_rn(__fmul_rn(fmaxf(hi - least_f, 0.f), 1.0f / 15.0f));
     const float scale_f = __half2float(scale);
     pair = (uint32_t)__half_as_ushort(scale) | ((uint32_t)__half_as_ushort(least) << 16);
     word[0] = word[1] = 0;
-    if (!(scale_f > 0.f)) return;  // one value, or a NaN
+    if (scale_f == 0.f) return;  // one value, or a NaN
     const float inv = __frcp_rn(scale_f);
     auto quotient = [&](float v) {
         const float t = v - least_f, q = t * inv;
