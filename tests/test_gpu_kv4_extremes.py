@@ -1,8 +1,10 @@
-"""The 4-bit cache at the ends of what it holds: constants that fp16 rounds up."""
+"""The 4-bit cache at the ends of what it holds: constants that fp16 rounds up, infinities."""
+import math
+
 import pytest
 import torch
 
-from tests.test_gpu_kv4 import _check_attention, _filled, _reference
+from tests.test_gpu_kv4 import _check_attention, _filled, _reference, _table
 
 pytestmark = pytest.mark.gpu
 
@@ -36,4 +38,38 @@ def test_constants_that_fp16_rounds_up(cuda_device, d, dtype):
                 q = torch.randn(rows, 4, d, generator=torch.Generator().manual_seed(n)).to(dtype).to(cuda_device)
                 got = ops.kv4_attention(q, cache, table, _dev([n], cuda_device), _dev([0, rows], cuda_device), rows, d ** -0.5)
                 _check_attention(got, _reference(q, cache, table, [n], [0, rows], d ** -0.5), f"{constant} {constants} {others} {rows}", halves=rows > 8)
+    assert lib.tc_status() == 0
+
+
+@pytest.mark.parametrize("beside", ["zeros", "ordinary", "the other infinity", "60000 below"])
+@pytest.mark.parametrize("d,group", [(64, 2), (128, 4), (256, 1)])
+@pytest.mark.parametrize("new,at", [(5, 3), (90, 70), (300, 299), (300, 0)])
+def test_infinities_are_held_as_the_largest_values(cuda_device, d, group, new, at, beside):
+    """Keys or values of one new token and one head hold an infinity. Code 15 of such a group may stand for more than fp16 holds: rows
+    before the token are what they are without it, rows from it on are finite and see the value."""
+    from xpu_graph_b200 import lib, ops
+
+    n, page, heads = new + 50, 32, 2
+    table, lens, starts = _table([n], page, 12, cuda_device), _dev([n], cuda_device), _dev([0, new], cuda_device)
+    q = torch.randn(new, heads * group, d, generator=torch.Generator().manual_seed(d)).bfloat16().to(cuda_device)
+    token = 50 + at
+    slot = table[0, token // page] * page + token % page
+    g = torch.Generator(cuda_device).manual_seed(1)
+    for side in ("keys", "values"):
+        cache = _filled(12, heads, page, d, cuda_device)
+        k, v = (torch.randn(1, heads, d, generator=g, device=cuda_device) for _ in range(2))
+        x = k if side == "keys" else v
+        if beside == "zeros":
+            x[0, 1, d - 64:] = 0
+        x[0, 1, d - 3] = math.inf
+        if beside == "the other infinity":
+            x[0, 1, d - 9] = -math.inf
+        if beside == "60000 below":
+            x[0, 1, d - 9] = -60000.0
+        ops.kv4_append(cache, k, v, slot[None])
+        got = ops.kv4_attention(q, cache, table, lens, starts, new, d ** -0.5)
+        assert torch.isfinite(got).all(), side
+        _check_attention(got, _reference(q, cache, table, [n], [0, new], d ** -0.5), side, halves=new > 8)
+        if side == "values":
+            assert (got[at:, group:, d - 3].abs() > 1.0).any()
     assert lib.tc_status() == 0

@@ -76,6 +76,31 @@ __device__ __forceinline__ uint4 unpack8(uint32_t w, __half2 scale, __half2 leas
     return make_uint4(out[0], out[1], out[2], out[3]);
 }
 
+// A scale that was rounded up may put code 15 (no other) beyond fp16's largest value, which is what such a code stands for: the infinity
+// that unpack8 makes of it would be NaN in the rows that do not see the token. It takes a scale of 4096 or more (half a step of a smaller
+// one is 1 at most, and 15 of those stay below the 16 between 65504 and what rounds to infinity). A warp that meets one goes over the
+// operand rows that it has stored once more: `rows` rows of 128 bytes, `groups` times, a block of keys apart. What asking costs, by a
+// packed maximum of the pairs' bits and a vote per block: 461 -> 468 us (3 sequences with 2048 new tokens), head dim 64 402 -> 406, 256
+// none; a test at every store cost 10 %.
+constexpr unsigned short kOverflowScale = 0x6c00;
+__device__ __noinline__ void end_at_largest(uint32_t base, int rows, int groups, int lane) {
+    __syncwarp();
+    const __half2 largest = __half2half2(__ushort_as_half(0x7bff));
+#pragma unroll 1
+    for (int i = lane; i < groups * rows * 8; i += 32) {
+        const int gr = i / (rows * 8);
+        const uint32_t at = base + (uint32_t)(gr * (PN * 128) + (i - gr * rows * 8) * 16);
+        uint4 v = ptx::ld_shared_v4(at);
+        uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const __half2 x = __hmin2_nan(*reinterpret_cast<const __half2*>(&w[e]), largest);
+            w[e] = *reinterpret_cast<const uint32_t*>(&x);
+        }
+        ptx::st_shared_v4(at, v);
+    }
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const AttendParams p, int beyond, const Parts parts) {
     using Cfg = PreCfg<D>;
@@ -253,6 +278,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
             const int there = hole ? 0 : u.len - ((j0 + j) * kBlockTiles + mine) * kTileTokens - h * Cfg::TOKENS;  // of this warp's tokens
             if (!__all_sync(0xffffffffu, ptx::mbar_wait_bounded(&k_empty[buf], ph ^ 1u, abort_flag))) { ok = false; break; }
             if (lane == 0) holes[(j & 3) * UNPACK + warp] = hole;
+            uint32_t top = 0;  // low half: largest scale that this lane looks at, by its bits
+            bool wide;
             {
                 const uint32_t base = ptx::smem_u32(k_s + buf * Cfg::KV_BYTES) + (uint32_t)(warp * Cfg::TOKENS * 128);
 #pragma unroll
@@ -264,7 +291,10 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
                     load_pairs<GR>(pair_s + r * (D / 16), pairs);
                     load_pairs<GR>(pair_s + P + r * (D / 16), v_pairs);
 #pragma unroll
-                    for (int gr = 0; gr < GR; ++gr) pairs[0] = __hfma2(v_pairs[gr], zero, pairs[0]);  // NaN if the token's values hold one
+                    for (int gr = 0; gr < GR; ++gr) {
+                        top = __vimax3_s16x2(top, *reinterpret_cast<const uint32_t*>(&pairs[gr]), *reinterpret_cast<const uint32_t*>(&v_pairs[gr]));
+                        pairs[0] = __hfma2(v_pairs[gr], zero, pairs[0]);  // NaN if the token's values hold one
+                    }
 #pragma unroll
                     for (int gr = 0; gr < GR; ++gr) {
                         const __half2 pair = r < there ? pairs[gr] : zero, scale = __low2half2(pair), least = __high2half2(pair);
@@ -273,6 +303,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
                             ptx::st_shared_v4(base + (uint32_t)(gr * (PN * 128) + r * 128 + (((4 * w + kt) ^ (r & 7)) << 4)), unpack8(words[2 * gr + w], scale, least));
                     }
                 }
+                wide = __any_sync(0xffffffffu, (int)(short)(top & 0xffffu) >= kOverflowScale);
+                if (wide) end_at_largest(base, Cfg::TOKENS, GR, lane);
             }
             ptx::fence_proxy_async();
             __syncwarp();
@@ -297,6 +329,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
                                           unpack8(words[w], __low2half2(pair), __high2half2(pair)));
                     }
                 }
+                if (wide) end_at_largest(base, Cfg::TOKENS, GR, lane);
             }
             ptx::fence_proxy_async();
             __syncwarp();
