@@ -366,7 +366,7 @@ int xg_qk_norm_rope(const void* q, const void* k, const void* q_weight, const vo
  * xg_kv4_append quantises tokens into slots: least = fp16(min x), scale = fp16(max(max x - least, 0) * fp32(1/15)),
  * code = rint((x - least) / scale) in 0..15 (0 where scale is 0) per token, head and 64 channels, fp32 with IEEE rounding. k, v:
  * [tokens, heads, D] by element strides. Values beyond +-65504 (infinities too) are held as that (where the
- * scale is rounded up, code * scale + least may pass it by up to 64; operands in fp16 end at it), a group with a NaN reads back as NaN. A slot outside the cache (-1, say, for padding rows) is skipped.
+ * scale is rounded up, code * scale + least may pass it by up to 64; fp16 operands and results end at it), a group with a NaN reads back as NaN. A slot outside the cache (-1, say, for padding rows) is skipped.
  * Slots are distinct; where two rows share one, that token's contents are unspecified. Nothing else in the cache is touched.
  * xg_kv4_read writes the slots' values to contiguous [tokens, heads, D]; a slot outside the cache reads as zeros.
  * xg_copy_pages copies page src[i] to page dst[i], any memory of `pages` pages of page_bytes (a multiple of 16). src, dst: HOST

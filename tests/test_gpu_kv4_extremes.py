@@ -1,10 +1,10 @@
-"""The 4-bit cache at the ends of what it holds: constants that fp16 rounds up, infinities."""
+"""The 4-bit cache at the ends of what it holds: constants that fp16 rounds up, infinities in operands and results."""
 import math
 
 import pytest
 import torch
 
-from tests.test_gpu_kv4 import _check_attention, _filled, _reference, _table
+from tests.test_gpu_kv4 import _check_attention, _filled, _reference, _same, _table
 
 pytestmark = pytest.mark.gpu
 
@@ -73,3 +73,38 @@ def test_infinities_are_held_as_the_largest_values(cuda_device, d, group, new, a
         if side == "values":
             assert (got[at:, group:, d - 3].abs() > 1.0).any()
     assert lib.tc_status() == 0
+
+
+def test_infinities_read_back_in_fp16(cuda_device):
+    """fp16 results end at fp16's largest value, where the same codes and scales stand for more in fp32."""
+    from xpu_graph_b200 import ops
+
+    x = torch.randn(6, 2, 128, generator=torch.Generator().manual_seed(0))
+    x[0, 0, 3], x[1, 1, 70], x[2, 0, 5], x[2, 0, 6], x[3, 1, 0] = math.inf, -math.inf, math.inf, -math.inf, math.nan
+    x[4, 0, :64] = 0
+    x[4, 0, 9] = math.inf
+    x = x.to(cuda_device)
+    cache = torch.zeros(1, 2, 1, 18 * 128, dtype=torch.uint8, device=cuda_device)
+    slots = torch.arange(6, device=cuda_device)
+    ops.kv4_append(cache, x, x.flip(0), slots)
+    for got, full in zip(ops.kv4_read(cache, slots, torch.float16), ops.kv4_read(cache, slots, torch.float32)):
+        assert not torch.isinf(got).any() and (full > 65520).any()
+        assert _same(got, full.clamp(-65504.0, 65504.0).half())
+
+
+@pytest.mark.parametrize("d,group", [(64, 2), (128, 4), (256, 1)])
+@pytest.mark.parametrize("new", [1, 7, 90])
+@pytest.mark.parametrize("sharp", [1.0, 4.0, 16.0])
+def test_averages_of_infinities_in_fp16(cuda_device, d, group, new, sharp):
+    """Rows whose weight lies on tokens with infinite values: the largest value, of either sign, by both kernels."""
+    from xpu_graph_b200 import ops
+
+    n = 200
+    x = torch.zeros(n, 2, d, device=cuda_device)
+    x[:, 0, ::2], x[:, 0, 1::2], x[:, 1, 5] = math.inf, -math.inf, math.inf
+    cache = torch.zeros(7, 2, 2, 18 * d, dtype=torch.uint8, device=cuda_device)
+    ops.kv4_append(cache, torch.randn(n, 2, d, generator=torch.Generator().manual_seed(0)).to(cuda_device), x, torch.arange(n, device=cuda_device))
+    q = torch.randn(new, 2 * group, d, generator=torch.Generator().manual_seed(1)).half().to(cuda_device)
+    got = ops.kv4_attention(q, cache, torch.arange(7, device=cuda_device)[None], _dev([n], cuda_device), _dev([0, new], cuda_device), new, sharp * d ** -0.5).float()
+    # weights that add to 1 within 200 roundings of 2^-11 at most, and fp32 sums
+    assert ((got - x.repeat_interleave(group, 1)[:1].clamp(-65504, 65504)).abs() <= 2.0 ** -11 * 65504 * 2).all()

@@ -47,13 +47,13 @@ __device__ __forceinline__ Sequence sequence(const AttendParams& p, int b) {
     return s;
 }
 
-// 8 channels of a finished row; a row that saw no key is zeros.
+// 8 channels of a finished row; a row that saw no key is zeros. (in_range: an average of the largest values may be rounded beyond them.)
 template <typename T>
 __device__ __forceinline__ void store_row8(T* out, const float (&o)[8], float sum) {
     const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
     Vec16<T> y;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y.v[e] = Cvt<T>::from_f(o[e] * inv);
+    for (int e = 0; e < 8; ++e) y.v[e] = Cvt<T>::from_f(in_range<T>(o[e] * inv));
     st16(out, y);
 }
 

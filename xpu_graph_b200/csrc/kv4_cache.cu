@@ -43,11 +43,6 @@ __device__ __forceinline__ Raw8<T> load8(const T* p) {
     return r;
 }
 
-__device__ __forceinline__ float min_nan(float a, float b) {  // NaN if one of them is
-    float y;
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
-    return y;
-}
 // Least (NaN where there is one) and largest of 8 values.
 __device__ __forceinline__ void extremes(const Raw8<float>& x, float& lo, float& hi) {
     lo = hi = x.v[0];
@@ -184,6 +179,11 @@ __device__ __forceinline__ void store_values(T* out, uint32_t word, uint32_t pai
         const uint32_t u = (word >> (8 * (i / 2))) & ((i & 1) ? 0x00f000f0u : 0x000f000fu);
         const float2 n = __half22float2(*reinterpret_cast<const __half2*>(&u));
         ptx::fma2(v[i], v[i + 4], n.x, n.y, (i & 1) ? odd : even, (i & 1) ? odd : even, least, least);
+    }
+    if constexpr (std::is_same<T, __half>::value) {  // (a smaller scale cannot be rounded up so far: kv4_tile.cuh)
+        if (scale >= kOverflowScale)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = in_range<T>(v[i]);
     }
     if constexpr (sizeof(T) == 2) {
         *reinterpret_cast<uint4*>(out) = make_uint4(ptx::pack2<T>(v[0], v[1]), ptx::pack2<T>(v[2], v[3]), ptx::pack2<T>(v[4], v[5]), ptx::pack2<T>(v[6], v[7]));

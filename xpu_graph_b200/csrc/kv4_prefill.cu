@@ -76,13 +76,11 @@ __device__ __forceinline__ uint4 unpack8(uint32_t w, __half2 scale, __half2 leas
     return make_uint4(out[0], out[1], out[2], out[3]);
 }
 
-// A scale that was rounded up may put code 15 (no other) beyond fp16's largest value, which is what such a code stands for: the infinity
-// that unpack8 makes of it would be NaN in the rows that do not see the token. It takes a scale of 4096 or more (half a step of a smaller
-// one is 1 at most, and 15 of those stay below the 16 between 65504 and what rounds to infinity). A warp that meets one goes over the
-// operand rows that it has stored once more: `rows` rows of 128 bytes, `groups` times, a block of keys apart. What asking costs, by a
-// packed maximum of the pairs' bits and a vote per block: 461 -> 468 us (3 sequences with 2048 new tokens), head dim 64 402 -> 406, 256
-// none; a test at every store cost 10 %.
-constexpr unsigned short kOverflowScale = 0x6c00;
+// The infinity that unpack8 makes of a code beyond fp16's largest value (kOverflowScale) would be NaN in the rows that do not see the
+// token. A warp that meets such a scale goes over the operand rows that it has stored once more: `rows` rows of 128 bytes, `groups`
+// times, a block of keys apart. What asking costs, by a packed maximum of the pairs' bits and a vote per block: 461 -> 468 us (3
+// sequences with 2048 new tokens), head dim 64 402 -> 406, 256 none; a test at every store cost 10 %.
+constexpr int kOverflowBits = 0x6c00;  // kOverflowScale in fp16
 __device__ __noinline__ void end_at_largest(uint32_t base, int rows, int groups, int lane) {
     __syncwarp();
     const __half2 largest = __half2half2(__ushort_as_half(0x7bff));
@@ -303,7 +301,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
                             ptx::st_shared_v4(base + (uint32_t)(gr * (PN * 128) + r * 128 + (((4 * w + kt) ^ (r & 7)) << 4)), unpack8(words[2 * gr + w], scale, least));
                     }
                 }
-                wide = __any_sync(0xffffffffu, (int)(short)(top & 0xffffu) >= kOverflowScale);
+                wide = __any_sync(0xffffffffu, (int)(short)(top & 0xffffu) >= kOverflowBits);
                 if (wide) end_at_largest(base, Cfg::TOKENS, GR, lane);
             }
             ptx::fence_proxy_async();
@@ -601,7 +599,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {  // channels 2 x, 2 x + 1 (unpack8's order)
                         const int at = t4 * 8 + 4 * (x & 1) + (x >> 1);
-                        w[x] = ptx::pack2<T>(__uint_as_float(o[at]) * inv_l, __uint_as_float(o[at + 2]) * inv_l);
+                        w[x] = ptx::pack2<T>(in_range<T>(__uint_as_float(o[at]) * inv_l), in_range<T>(__uint_as_float(o[at + 2]) * inv_l));
                     }
                     const int at = (c & 1) * 4 + t4;
                     ptx::st_shared_v4(slab + (uint32_t)(lane * 128 + ((at ^ (lane & 7)) << 4)), make_uint4(w[0], w[1], w[2], w[3]));
@@ -666,7 +664,7 @@ __global__ void __launch_bounds__(256) kv4_prefill_combine_kernel(const AttendPa
     // column x of 8 is channel 4 (x & 1) + x / 2 (unpack8's order)
     const int ch = (lane & ~7) + 4 * (lane & 1) + ((lane & 7) >> 1);
 #pragma unroll
-    for (int c = 0; c < C; ++c) out[c * 32 + ch] = Cvt<T>::from_f(o[c] * inv);
+    for (int c = 0; c < C; ++c) out[c * 32 + ch] = Cvt<T>::from_f(in_range<T>(o[c] * inv));
 }
 
 // The most units there can be, and over how many CTAs each one's keys are shared out: as many as fill the chip once, 320 keys or more each

@@ -18,11 +18,33 @@
 
 #include "common.cuh"
 
+#include <type_traits>
+
 namespace xg {
 namespace kv4 {
 
 constexpr int kTileTokens = 16;
 constexpr float kLargest = 65504.0f;  // of fp16: values beyond are held as it
+// A scale that was rounded up may put code 15 (no other) beyond kLargest, which is what such a code stands for: fp16 operands and results
+// end there. To pass it so far that fp16 rounds to infinity (16 above it) takes a scale of 4096 or more: half a step of a smaller one
+// is 1 at most, 15 times.
+constexpr float kOverflowScale = 4096.0f;
+
+__device__ __forceinline__ float min_nan(float a, float b) {  // NaN if one of them is
+    float y;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+
+// fp16 results end at fp16's largest value (a NaN stays one); other types hold what there is.
+template <typename T>
+__device__ __forceinline__ float in_range(float x) {
+    if constexpr (std::is_same<T, __half>::value) {
+        x = min_nan(x, kLargest);
+        asm("max.NaN.f32 %0, %1, %2;" : "=f"(x) : "f"(x), "f"(-kLargest));
+    }
+    return x;
+}
 
 __host__ __device__ constexpr int tile_bytes(int D) { return 18 * D; }
 
