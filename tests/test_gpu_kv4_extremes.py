@@ -1,4 +1,5 @@
-"""The 4-bit cache at the ends of what it holds: constants that fp16 rounds up, infinities in operands and results."""
+"""The 4-bit cache at the ends of what it holds: constants that fp16 rounds up, infinities in operands and results, weights far below
+the largest."""
 import math
 
 import pytest
@@ -108,3 +109,27 @@ def test_averages_of_infinities_in_fp16(cuda_device, d, group, new, sharp):
     got = ops.kv4_attention(q, cache, torch.arange(7, device=cuda_device)[None], _dev([n], cuda_device), _dev([0, new], cuda_device), new, sharp * d ** -0.5).float()
     # weights that add to 1 within 200 roundings of 2^-11 at most, and fp32 sums
     assert ((got - x.repeat_interleave(group, 1)[:1].clamp(-65504, 65504)).abs() <= 2.0 ** -11 * 65504 * 2).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("rows", [60, 70])  # (up to 64 are streamed at head dim 64)
+def test_many_keys_far_below_the_largest_score(cuda_device, rows, d, dtype):
+    """One key 17.5 above 16383 others, whose weights of e^-17.5 make 0.04 % of the sum and, as the first value is 0, all of the result.
+    A weight of 2^-18.2 beside a largest of 2^7 is 54 steps of fp16's smallest, half a step off at most: 2^-6.7. The result's own
+    rounding is 2^-8 at most, the sums add less than 2^-12."""
+    from xpu_graph_b200 import ops
+
+    n = 16384
+    cache = torch.zeros(n // 64, 1, 4, 18 * d, dtype=torch.uint8, device=cuda_device)
+    k, v = torch.zeros(n, 1, d, device=cuda_device), torch.ones(n, 1, d, device=cuda_device)
+    k[0], v[0] = 1.0, 0.0
+    ops.kv4_append(cache, k, v, torch.arange(n, device=cuda_device))
+    table = torch.arange(n // 64, device=cuda_device)[None]
+    for around in (0, 150 * 256):  # rows of no sequence, with which the keys stay in one piece
+        q = torch.ones(rows + around, 1, d, device=cuda_device, dtype=dtype)
+        got = ops.kv4_attention(q, cache, table, _dev([n], cuda_device), _dev([0, rows], cuda_device), rows, 17.5 / d)[:rows, 0].double()
+        weight = (n - rows + torch.arange(rows, device=cuda_device)[:, None].double()) * math.exp(-17.5)
+        want = weight / (1 + weight)
+        tol = 2.0 ** -32 / math.exp(-17.5) + torch.finfo(dtype).eps / 2 + 2.0 ** -12
+        assert ((got - want).abs() <= tol * want).all(), (around, (got / want).amin().item(), (got / want).amax().item())
