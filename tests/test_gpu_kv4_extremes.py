@@ -1,5 +1,5 @@
-"""The 4-bit cache at the ends of what it holds: constants that fp16 rounds up, infinities in operands and results, weights far below
-the largest."""
+"""The 4-bit cache at the ends of what it holds: constants that fp16 rounds up, infinities in operands and results, weights and
+query channels far below the largest."""
 import math
 
 import pytest
@@ -133,3 +133,23 @@ def test_many_keys_far_below_the_largest_score(cuda_device, rows, d, dtype):
         want = weight / (1 + weight)
         tol = 2.0 ** -32 / math.exp(-17.5) + torch.finfo(dtype).eps / 2 + 2.0 ** -12
         assert ((got - want).abs() <= tol * want).all(), (around, (got / want).amin().item(), (got / want).amax().item())
+
+
+@pytest.mark.parametrize("new", [3, 70])
+def test_a_channel_far_above_the_others(cuda_device, new):
+    """fp16 queries with one channel 2^23 times the others', where the keys are zero: the others make the scores."""
+    from xpu_graph_b200 import ops
+
+    d, n = 128, 300
+    g = torch.Generator().manual_seed(0)
+    cache = torch.zeros(10, 2, 2, 18 * d, dtype=torch.uint8, device=cuda_device)
+    k, v = torch.randn(320, 2, d, generator=g) * 500, torch.randn(320, 2, d, generator=g)
+    k[..., :64] = 0
+    ops.kv4_append(cache, k.to(cuda_device), v.to(cuda_device), torch.arange(320, device=cuda_device))
+    q = torch.randn(new, 4, d, generator=g) * 2.0 ** -8
+    q[..., :64] = 0
+    q[..., 7] = 2.0 ** 15
+    q = q.half().to(cuda_device)
+    table = torch.arange(10, device=cuda_device)[None]
+    got = ops.kv4_attention(q, cache, table, _dev([n], cuda_device), _dev([0, new], cuda_device), new, 0.5)
+    _check_attention(got, _reference(q, cache, table, [n], [0, new], 0.5), "scores of small channels", halves=new > 8)

@@ -6,9 +6,9 @@
 // tiles into double-buffered tensor memory, then O += P V with P read from tensor memory; eight warps (a row per thread) turn
 // scores into probabilities in place, as flash_tc_kernel (sdpa.cu) does, with the maximum lagging by up to 2^8.
 //
-// Everything that meets in a product is fp16: codes are exact there, code * scale + least is rounded once (2^-12 relative), as are
-// probabilities; fp16 queries stay as they are and bf16 ones too, after a power of two per row has been taken out (it returns in the
-// row's exponent factor). Sums are fp32 in tensor memory and registers.
+// Everything that meets in a product is fp16: codes are exact there, code * scale + least is rounded once (2^-11 relative), as are
+// probabilities (kTop). Queries are carried after a power of two per row, the row's largest below 2^15, which returns in the row's
+// exponent factor: exactly, down to 2^-29 of that largest. Sums are fp32 in tensor memory and registers.
 //
 // What bounds it: per block of 64 keys the products take 1024 cycles of the tensor pipe (41 % busy), the 256 x 64 exponentials 1024 of
 // the special-function unit (41 %), and unpacking (2 operations per code) and softmax 49 % of the issue slots; they run beside each
@@ -438,12 +438,11 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const A
                     for (int x = 0; x < 8; ++x) top = fmaxf(top, fabsf(Cvt<T>::to_f(e[x])));
                 }
             }
-            int e = (int)(__float_as_uint(top) >> 23) - 127;
-            e = max(-100, min(126, e));
-            float down = __uint_as_float((uint32_t)(127 - e) << 23);
+            const int e = max(-100, (int)(__float_as_uint(top) >> 23) - 127);  // the row is carried below 2^15 (up to 128: infinities)
+            float down = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
             if (p.scale == 0.f) down = 0.f;
             if (p.scale < 0.f) down = -down;
-            mul = fmaxf((p.scale == 0.f ? 1.f : fabsf(p.scale)) * kLog2e * __uint_as_float((uint32_t)(127 + e) << 23), 1e-37f);
+            mul = fmaxf((p.scale == 0.f ? 1.f : fabsf(p.scale)) * kLog2e * __uint_as_float((uint32_t)(127 + e - 14) << 23), 1e-37f);
             const uint32_t base = ptx::smem_u32(q_s + i * Cfg::Q_BYTES) + (uint32_t)(r_in_tile * 128);
 #pragma unroll
             for (int c0 = D / 8 - HELD; c0 >= 0; c0 -= HELD) {
