@@ -153,3 +153,18 @@ def test_a_channel_far_above_the_others(cuda_device, new):
     table = torch.arange(10, device=cuda_device)[None]
     got = ops.kv4_attention(q, cache, table, _dev([n], cuda_device), _dev([0, new], cuda_device), new, 0.5)
     _check_attention(got, _reference(q, cache, table, [n], [0, new], 0.5), "scores of small channels", halves=new > 8)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("new", [3, 90])
+def test_rows_of_any_size(cuda_device, d, new):
+    """bf16 queries near the ends of what the type holds, with a scale that makes scores of ordinary size of them."""
+    from xpu_graph_b200 import ops
+
+    n = 300
+    cache = _filled(10, 2, 32, d, cuda_device)
+    table = torch.arange(10, device=cuda_device)[None]
+    q = torch.randn(new, 4, d, generator=torch.Generator().manual_seed(d)).bfloat16().to(cuda_device)
+    for power in (2.0 ** 99, 2.0 ** 103, 2.0 ** 112, 2.0 ** 122, 2.0 ** -95):
+        got = ops.kv4_attention(q * power, cache, table, _dev([n], cuda_device), _dev([0, new], cuda_device), new, d ** -0.5 / power)
+        _check_attention(got, _reference(q * power, cache, table, [n], [0, new], d ** -0.5 / power), f"{power}", halves=new > 8)

@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
                 }
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const int e2 = max(-100, min(100, (int)(__float_as_uint(top) >> 23) - 127));  // the row is carried below 2^15
+                const int e2 = max(-100, (int)(__float_as_uint(top) >> 23) - 127);  // the row is carried below 2^15 (up to 128: infinities)
                 const float up = q_mul * __uint_as_float((uint32_t)(127 + 14 - e2) << 23);
 #pragma unroll
                 for (int gr = 0; gr < GR; ++gr) {
@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(kWarps * 32, (SplitCfg<D, NT>::CTAS)) kv4_spli
 #pragma unroll
                     for (int c = 0; c < 2; ++c) qsum[nt][gr][c] = 0x1p-24f * __shfl_sync(0xffffffffu, sum, (2 * t + c) * 4);
                 }
-                const float back = fmaxf(scale_log2 * __uint_as_float((uint32_t)(127 + 10 + e2) << 23), 1e-37f);
+                const float back = fmaxf(scale_log2 * __uint_as_float((uint32_t)(127 - 20 + e2) << 23) * 0x1p30f, 1e-37f);
                 const int lim = on ? len - count + token + 1 : 0x7fffffff;  // keys that the column sees
                 least_limit = min(least_limit, lim);
 #pragma unroll
