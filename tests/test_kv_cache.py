@@ -98,3 +98,23 @@ def test_any_order_of_them_keeps_every_sequence(cache):
 def test_refusals(bad):
     with pytest.raises(ValueError):
         kv_cache.KV4Cache(**{**dict(pages=4, kv_heads=1, head_dim=64, device="cpu"), **bad})
+
+
+def test_a_fork_that_fails_leaves_the_pages_free(cache, monkeypatch):
+    a = cache.new()
+    cache.extend(a, 20)
+    free, working = cache.free_pages, kv_cache.ops.copy_pages
+
+    def failing(t, src, dst):
+        raise RuntimeError("no copy")
+
+    monkeypatch.setattr(kv_cache.ops, "copy_pages", failing)
+    for _ in range(20):  # more often than there are pages
+        with pytest.raises(RuntimeError, match="no copy"):
+            cache.fork(a)
+    assert cache.free_pages == free and cache.pages(a) == (0, 1)
+    monkeypatch.setattr(kv_cache.ops, "copy_pages", working)
+    b = cache.fork(a)
+    assert cache.pages(b)[0] == 0 and cache.free_pages == free - 1
+    cache.free(a), cache.free(b)
+    assert cache.free_pages == 12

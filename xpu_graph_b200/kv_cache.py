@@ -77,7 +77,11 @@ class KV4Cache:
         pages, n = self._pages[seq], self._length[seq]
         full = n // self.page_size
         own = self._take(len(pages) - full)  # (before anything is changed)
-        self._copy(pages[full:], own)
+        try:
+            self._copy(pages[full:], own)
+        except BaseException:
+            self._drop(own)
+            raise
         for p in pages[:full]:
             self._holders[p] += 1
         twin = self.new()
