@@ -118,3 +118,24 @@ def test_a_fork_that_fails_leaves_the_pages_free(cache, monkeypatch):
     assert cache.pages(b)[0] == 0 and cache.free_pages == free - 1
     cache.free(a), cache.free(b)
     assert cache.free_pages == 12
+
+
+def test_an_extension_that_fails_changes_nothing(cache, monkeypatch):
+    """The slots' tensor may fail to be made: the sequence is no longer than before, and its pages are free."""
+    a = cache.new()
+    cache.extend(a, 20)
+
+    class Full:
+        def __init__(self, *args, **kwargs):
+            pass
+
+        def to(self, *args, **kwargs):
+            raise RuntimeError("out of memory")
+
+    with monkeypatch.context() as m:
+        m.setattr(kv_cache.torch, "tensor", Full)
+        for _ in range(20):
+            with pytest.raises(RuntimeError, match="out of memory"):
+                cache.extend(a, 30)
+    assert cache.length(a) == 20 and cache.pages(a) == (0, 1) and cache.free_pages == 10
+    assert cache.extend(a, 13).tolist() == list(range(20, 33)) and cache.pages(a) == (0, 1, 2)

@@ -67,10 +67,17 @@ class KV4Cache:
         if tokens < 0:
             raise ValueError("KV4Cache: a negative number of tokens")
         pages, n, size = self._pages[seq], self._length[seq], self.page_size
-        pages += self._take(-(-(n + tokens) // size) - len(pages))
+        held = len(pages)
+        pages += self._take(-(-(n + tokens) // size) - held)
+        try:
+            slots = torch.tensor([pages[i // size] * size + i % size for i in range(n, n + tokens)], dtype=torch.int64)
+            slots = slots.to(self.layers[0].device, non_blocking=True)
+        except BaseException:
+            self._drop(pages[held:][::-1])
+            del pages[held:]
+            raise
         self._length[seq] = n + tokens
-        slots = torch.tensor([pages[i // size] * size + i % size for i in range(n, n + tokens)], dtype=torch.int64)
-        return slots.to(self.layers[0].device, non_blocking=True)
+        return slots
 
     def fork(self, seq: int) -> int:
         """Another sequence with the same tokens. Full pages are shared; the last one, if it is not full, is copied."""
@@ -80,7 +87,7 @@ class KV4Cache:
         try:
             self._copy(pages[full:], own)
         except BaseException:
-            self._drop(own)
+            self._drop(own[::-1])
             raise
         for p in pages[:full]:
             self._holders[p] += 1
