@@ -111,3 +111,10 @@ def test_a_row_for_each_sequence_where_there_are_no_starts():
         assert attend(tokens, batch, max_q) == -1, (tokens, batch, max_q)
         assert "row" in lib.last_error()
     assert attend(0, 2, 1) == 0
+
+
+def test_page_lists_under_another_default_device():
+    for n in (0, 2, 300):
+        with torch.device("meta"):
+            got = ops._host_ints(list(range(n)))
+        assert got.device.type == "cpu" and torch.equal(got, torch.arange(n))

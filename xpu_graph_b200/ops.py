@@ -544,7 +544,7 @@ def _host_ints(v) -> torch.Tensor:
     if isinstance(v, torch.Tensor):
         return v
     if len(v) < 256:  # the library's loop is the faster one from there on (1500 numbers: 5 us, an array 13), its call the slower one below
-        return torch.frombuffer(array.array("q", v), dtype=torch.int64) if len(v) else torch.empty(0, dtype=torch.int64)
+        return torch.frombuffer(array.array("q", v), dtype=torch.int64) if len(v) else torch.empty(0, dtype=torch.int64, device="cpu")
     t = torch.empty(len(v), dtype=torch.int64, device="cpu")
     _lib.load_torch_ops().xg_torch_ints(v, t.data_ptr(), len(v))  # raises what the call sets
     return t
