@@ -118,3 +118,16 @@ def test_page_lists_under_another_default_device():
         with torch.device("meta"):
             got = ops._host_ints(list(range(n)))
         assert got.device.type == "cpu" and torch.equal(got, torch.arange(n))
+
+
+@pytest.mark.parametrize("n", [0, 2, 300])
+def test_copy_pages_of_a_fake_cache(n):
+    """Lists of any length with tensors that have no memory, as graph compilers trace them."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        cache = torch.empty(1000, 4, 16, device="cuda")
+        assert ops.copy_pages(cache, list(range(n)), range(n, 2 * n)) is None
+        for bad in ([1.5], ["1"] * 300):
+            with pytest.raises((TypeError, ValueError)):
+                ops.copy_pages(cache, bad, bad)

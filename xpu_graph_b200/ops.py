@@ -543,6 +543,8 @@ class _CopyPages(NativeOp):
 def _host_ints(v) -> torch.Tensor:
     if isinstance(v, torch.Tensor):
         return v
+    if torch._C._len_torch_dispatch_stack():  # a fake tensor has no memory to write to, and takes no real one beside it
+        return torch.tensor(array.array("q", v).tolist(), dtype=torch.int64, device="cpu")
     if len(v) < 256:  # the library's loop is the faster one from there on (1500 numbers: 5 us, an array 13), its call the slower one below
         return torch.frombuffer(array.array("q", v), dtype=torch.int64) if len(v) else torch.empty(0, dtype=torch.int64, device="cpu")
     t = torch.empty(len(v), dtype=torch.int64, device="cpu")
