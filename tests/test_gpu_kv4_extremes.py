@@ -168,3 +168,24 @@ def test_rows_of_any_size(cuda_device, d, new):
     for power in (2.0 ** 99, 2.0 ** 103, 2.0 ** 112, 2.0 ** 122, 2.0 ** -95):
         got = ops.kv4_attention(q * power, cache, table, _dev([n], cuda_device), _dev([0, new], cuda_device), new, d ** -0.5 / power)
         _check_attention(got, _reference(q * power, cache, table, [n], [0, new], d ** -0.5 / power), f"{power}", halves=new > 8)
+
+
+def test_few_pages_of_very_many(cuda_device):
+    """One page among 2^27: what the checks of the numbers take goes by the numbers, not by the pages (2^27 bytes cleared take 20 ms)."""
+    import time
+
+    from xpu_graph_b200 import ops
+
+    rows = torch.zeros(1 << 27, 16, dtype=torch.uint8, device=cuda_device)
+    last = (1 << 27) - 1
+    rows[last] = 7
+    took = []
+    for i in range(5):
+        since = time.perf_counter()
+        ops.copy_pages(rows, [last, last], [5 + i, 100 + i])
+        took.append(time.perf_counter() - since)
+    assert (rows[5:10] == 7).all() and (rows[100:105] == 7).all() and not rows[10:100].any() and not rows[:5].any()
+    assert min(took) < 2e-3
+    for src, dst in (([0, 1], [2, 2]), ([0, 1], [2, 0]), ([1 << 27], [0]), ([0], [-1])):
+        with pytest.raises(ValueError):
+            ops.copy_pages(rows, src, dst)

@@ -22,6 +22,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 #include <cstdlib>
@@ -861,15 +862,27 @@ void copy_pages(const Tensor& cache, const Tensor& src_in, const Tensor& dst_in)
     const int64_t bytes = pages > 0 ? cache.numel() / pages * (int64_t)cache.element_size() : 0;
     TORCH_CHECK_VALUE(pages == 0 || cache.select(0, 0).is_contiguous(), "xg_sm100::copy_pages: a page must be contiguous");
     const int64_t stride = pages > 1 ? cache.stride(0) * (int64_t)cache.element_size() : bytes;
-    std::vector<char> is_dst(pages, 0);
-    for (const int64_t d : dst) {
-        TORCH_CHECK_VALUE(d >= 0 && d < pages, "xg_sm100::copy_pages: no page ", d, " among ", pages);
-        TORCH_CHECK_VALUE(!is_dst[d], "xg_sm100::copy_pages: page ", d, " is a destination twice");
-        is_dst[d] = 1;
-    }
-    for (const int64_t s : src) {
-        TORCH_CHECK_VALUE(s >= 0 && s < pages, "xg_sm100::copy_pages: no page ", s, " among ", pages);
-        TORCH_CHECK_VALUE(!is_dst[s], "xg_sm100::copy_pages: page ", s, " is source and destination");
+    const auto there = [&](int64_t p) { TORCH_CHECK_VALUE(p >= 0 && p < pages, "xg_sm100::copy_pages: no page ", p, " among ", pages); };
+    const auto check = [&](const auto& twice, const auto& is_dst) {
+        for (const int64_t d : dst) {
+            there(d);
+            TORCH_CHECK_VALUE(!twice(d), "xg_sm100::copy_pages: page ", d, " is a destination twice");
+        }
+        for (const int64_t s : src) {
+            there(s);
+            TORCH_CHECK_VALUE(!is_dst(s), "xg_sm100::copy_pages: page ", s, " is source and destination");
+        }
+    };
+    // A byte per page is the faster table (1500 numbers: of 4096 pages 1.7 us, of 100000 4.2, sorted 277; 6 of 100000: 1.9 us, sorted 0.1) as
+    // long as there are not a thousand times more pages than numbers.
+    if (pages <= 4096 + 1024 * (int64_t)dst.size()) {
+        std::vector<char> seen(pages, 0);
+        check([&](int64_t d) { return std::exchange(seen[d], 1); }, [&](int64_t s) { return seen[s]; });
+    } else {
+        std::vector<int64_t> sorted(dst.begin(), dst.end());
+        std::sort(sorted.begin(), sorted.end());
+        check([&](int64_t d) { const auto r = std::equal_range(sorted.begin(), sorted.end(), d); return r.second - r.first > 1; },
+              [&](int64_t s) { return std::binary_search(sorted.begin(), sorted.end(), s); });
     }
     const On on(cache);
     XG_CALL(xg_copy_pages, mut(cache), pages, bytes, stride, src.data(), dst.data(), (int64_t)src.size(), on.stream);
