@@ -366,7 +366,8 @@ int xg_qk_norm_rope(const void* q, const void* k, const void* q_weight, const vo
  * xg_kv4_append quantises tokens into slots: least = fp16(min x), scale = fp16(max(max x - least, 0) * fp32(1/15)),
  * code = rint((x - least) / scale) in 0..15 (0 where scale is 0) per token, head and 64 channels, fp32 with IEEE rounding. k, v:
  * [tokens, heads, D] by element strides. Values beyond +-65504 (infinities too) are held as that (where the
- * scale is rounded up, code * scale + least may pass it by up to 64; fp16 operands and results end at it), a group with a NaN reads back as NaN. A slot outside the cache (-1, say, for padding rows) is skipped.
+ * scale is rounded up, code * scale + least may pass it by up to 64; fp16 operands and results end at it), a group with a NaN reads
+ * back as NaN. A slot outside the cache (-1, say, for padding rows) is skipped.
  * Slots are distinct; where two rows share one, that token's contents are unspecified. Nothing else in the cache is touched.
  * xg_kv4_read writes the slots' values to contiguous [tokens, heads, D]; a slot outside the cache reads as zeros.
  * xg_copy_pages copies page src[i] to page dst[i], any memory of `pages` pages of page_bytes (a multiple of 16). src, dst: HOST
@@ -384,14 +385,16 @@ int xg_copy_pages(void* base, int64_t pages, int64_t page_bytes, int64_t page_st
 /*
  * Attention of the newest tokens of every sequence over its pages: out = softmax(q k^T * scale) v.
  * q: [tokens, q_heads, D] by element strides per token and head; out: contiguous. Rows q_starts[b] .. q_starts[b+1] (device,
- * batch + 1 non-decreasing entries; null: row b alone, and no more sequences than rows) belong to sequence b, whose kv_lens[b] cached tokens include them: of its n
- * rows, row i sees the keys up to position kv_lens[b] - n + i. max_q: the most rows that a sequence has; it chooses the kernels (the
- * results are within rounding of each other, and any value is safe). Token j of sequence b lies in page page_table[b * table_stride +
- * j / page_size]; a page number outside the cache hides its keys. q_heads is a multiple of kv_heads, query head h reads kv head
- * h / (q_heads / kv_heads). Rows that see no key, and rows of no sequence, are zeros; a NaN in a key or a value makes NaN of the rows
- * that see it, and of no other. 16-bit dtypes. All index arrays are int64 device memory; lengths and starts out of range are clamped
- * to what there is (rows that starts going back leave out, or give twice, are unspecified). Workspace: xg_kv4_attention_workspace_bytes (max_len =
- * table_pages * page_size), 16-byte aligned; its contents before and after the call are unspecified.
+ * batch + 1 non-decreasing entries; null: row b alone, and no more sequences than rows) belong to sequence b, whose kv_lens[b] cached
+ * tokens include them: of its n rows, row i sees the keys up to position kv_lens[b] - n + i. max_q: the most rows that a sequence has;
+ * it chooses the kernels (the results are within rounding of each other - many rows read keys and values rounded to fp16, few rows the
+ * codes as they are - and any value is safe). Token j of sequence b lies in page page_table[b * table_stride + j / page_size]; a page
+ * number outside the cache hides its keys. q_heads is a multiple of kv_heads, query head h reads kv head h / (q_heads / kv_heads). Rows
+ * that see no key, and rows of no sequence, are zeros; a NaN in a key or a value makes NaN of the rows that see it, and of no other.
+ * Scores are taken to stay below 2^23 in size (larger ones are whole numbers in fp32): far beyond, a row may become NaN. 16-bit dtypes.
+ * All index arrays are int64 device memory; lengths and starts out of range are clamped to what there is (rows that starts going back
+ * leave out, or give twice, are unspecified). Workspace: xg_kv4_attention_workspace_bytes (max_len = table_pages * page_size), 16-byte
+ * aligned; its contents before and after the call are unspecified.
  * Reference counterpart: the same aten.scaled_dot_product_attention call site as xg_sdpa_fwd, for a cache it does not have.
  */
 int64_t xg_kv4_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t D, int64_t max_q,

@@ -26,8 +26,8 @@ using namespace kv4;
 // arithmetic.
 //   scores (16 keys x 8 columns, per group of 64 channels):  x = scale_k acc + least_k sum(q), the group's sum of q kept per column.
 //     q has a power of two per row taken out, with which bf16 fits fp16 exactly (down to 2^-29 of the row's largest).
-//   output (16 channels x 8 columns):  sum p v = sum w (code - 8) + sum p (least_v + 8 scale_v), w = p scale_v rounded to fp16 (2^-12
-//     relative). The codes go in as they are; 8 sum w, from a product with ones, comes off every 256 keys, before the sums have
+//   output (16 channels x 8 columns):  sum p v = sum w (code - 8) + sum p (least_v + 8 scale_v), w = p scale_v rounded to fp16 (2^-11
+//     relative at most). The codes go in as they are; 8 sum w, from a product with ones, comes off every 256 keys, before the sums have
 //     grown so far that what the tensor core cuts off below 2^-24 of them is a bias (a flat average over 131072 keys would be 3 % off).
 //     It cuts by the operands' exponents, which subnormals do not have: a code 2^-20 loses four bits less than one 2^-24. Where that
 //     shows, in fp16 results, both codes of a byte go in as 2^-20 (131072 keys: 0.00036 of the result, then 0.00030; 0.00021 is its
@@ -40,7 +40,8 @@ using namespace kv4;
 // blocks 64 sequences of 512 to 8192 tokens took 92 us, with one 82).
 // What bounds it: unpacking and the softmax's scalar work, 54 % of the issue slots and 48 % of the logic pipe at three warps a
 // scheduler, beside 50 % of HBM: 4 sequences of 65536, 32 / 8 heads of 128: 75 us, 4.05 TB/s (the loads alone 60, the arithmetic alone
-// 73). More tiles in work at once, other occupancies, packed fp32 pairs and shifts by multiplication gave nothing.
+// 73). More tiles in work at once, other occupancies, packed fp32 pairs and shifts by multiplication gave nothing. Not used: with one new
+// token and a group of 4, columns 4-7 do not exist, and the lanes that hold them do the softmax's work for nothing.
 constexpr int kWarps = 4;
 constexpr int kBlockTiles = 2, kBlockKeys = kBlockTiles * kTileTokens;  // what a stage holds
 constexpr int kMaxBatch = 1024;  // sequences per launch: their prefix sums live in shared memory

@@ -1,5 +1,7 @@
-// Keys and values in 4 bits: quantising new tokens into cache pages, reading tokens back, copying pages. All three move bytes and
-// are bound by HBM (the layout: kv4_tile.cuh).
+// Keys and values in 4 bits: quantising new tokens into cache pages, reading tokens back, copying pages (the layout: kv4_tile.cuh). All
+// three move bytes, so HBM is their floor. What bounds them now: a prompt's append and read are held up by issuing (65 and 70 % of the
+// slots at 28 and 19 % of DRAM; most of it is addresses and what every lane of a group does for the group), few tokens by the host,
+// page copies by the launches and their gaps.
 //
 // Quantising, per token, head and group of 64 channels: least = fp16(min x), scale = fp16(max(max x - least, 0) * fp32(1/15)),
 // code = rint((x - least) / scale) in 0..15 (0 where the scale is 0), every step in fp32 with IEEE rounding. The fp16 roundings of the
@@ -67,7 +69,7 @@ __device__ __forceinline__ void extremes(const Raw8<__half>& x, float& lo, float
 //
 // The quotients come from one correctly rounded reciprocal and a step of correction with an exact remainder, which gives the correctly
 // rounded quotient (Markstein, IBM J. Res. Dev. 34, 1990): three operations each in place of a division. Codes are gathered four at a
-// time in a float, off the logic pipe, and everything goes in pairs. What bounds it is issuing (70 % of the slots). 16384 tokens x 8
+// time in a float, off the logic pipe, and everything goes in pairs. What bounds it is issuing (65 % of the slots). 16384 tokens x 8
 // heads x 128 in bf16: divisions 63 us, one by one 30 us, this 28.5 us (3.0 TB/s).
 template <typename T>
 __device__ __forceinline__ void quantise(const Raw8<T> (&x)[2], uint32_t (&word)[2], uint32_t& pair) {
@@ -260,7 +262,7 @@ int launch_type(const TokenParams& p, int64_t D, int dtype, bool append, cudaStr
 
 // ---- pages ---------------------------------------------------------------------------------------
 // A launch's page numbers go with it: no copy to the device, and the caller's lists are free when the call returns. 1500 pages of 73 KB:
-// 42 us, 10.7 us a launch (6.2 TB/s) and the gaps between four.
+// 42 us, 10.7 us a launch (33 MB read, and as much written, most of which is still in L2 when it ends) and the gaps between four.
 constexpr int kPairs = 448;  // page pairs per launch: with the rest within 4 KiB of kernel parameters
 struct PageParams {
     uint8_t* base;

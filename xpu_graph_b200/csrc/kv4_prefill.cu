@@ -10,12 +10,13 @@
 // probabilities (kTop). Queries are carried after a power of two per row, the row's largest below 2^15, which returns in the row's
 // exponent factor: exactly, down to 2^-29 of that largest. Sums are fp32 in tensor memory and registers.
 //
-// What bounds it: per block of 64 keys the products take 1024 cycles of the tensor pipe (41 % busy), the 256 x 64 exponentials 1024 of
+// What bounds it: per block of 64 keys the products take 1024 cycles of the tensor pipe (40 % busy), the 256 x 64 exponentials 1024 of
 // the special-function unit (41 %), and unpacking (2 operations per code) and softmax 49 % of the issue slots; they run beside each
 // other, but a tile's scores, probabilities and product follow one another, and about 8 us in front of and behind a unit's blocks
-// overlap with nothing. 3 sequences of 2048 to 8192 keys with 2048 new tokens, 32 / 8 heads of 128: 0.475-0.49 ms, 990-1024 TFLOP/s. Tried without gain: a warpgroup more for unpacking with the
-// registers dealt out anew; the last wave's units shared out over the idle CTAs (their parts cost what the wave gains). Head dim 256
-// has room for one tile and one buffer of V: 566 TFLOP/s.
+// overlap with nothing. 3 sequences of 2500 to 8192 keys with 2048 new tokens: 32 / 8 heads of 128 464 us back to back (1047 TFLOP/s),
+// 500 with pauses, 564 on another machine; of 64 403 us (604 TFLOP/s). Head dim 256 has room for one tile and one buffer of V: 16 / 4 heads
+// 827 us (588 TFLOP/s). Tried without gain: a warpgroup more for unpacking with the registers dealt out anew; the last wave's units
+// shared out over the idle CTAs (their parts cost what the wave gains).
 #include "kv4_attend.cuh"
 
 namespace xg {

@@ -552,7 +552,7 @@ def _host_ints(v) -> torch.Tensor:
     return t
 
 
-# cache[dst[i]] = cache[src[i]] for pages of any tensor (dimension 0). No page is a destination twice, or source and destination.
+# cache[dst[i]] = cache[src[i]] for pages (dimension 0) of a multiple of 16 bytes of any tensor. No page is a destination twice, or source and destination.
 copy_pages = _CopyPages("copy_pages")
 
 
